@@ -62,7 +62,7 @@
 extern "C" {
 #endif
 
-#define RIA_ABI_VERSION 6
+#define RIA_ABI_VERSION 7
 
 enum ria_dtype { RIA_DT_BF16 = 0, RIA_DT_F16 = 1, RIA_DT_F32 = 2 };
 
@@ -698,6 +698,105 @@ int ria_linear_fp8_group(int m, int k, const void* x, int x_dtype, int64_t x_row
 int ria_linear_fp8_group_normed(int m, int k, const float* x, int64_t x_row_stride,
                                 const float* norm_weight, float eps, int h_dtype, int count,
                                 const ria_fp8_proj* projs, void* stream);
+
+/*
+ * The mixture-of-experts block that runs between the attention layers
+ * (qwen36_chat_batch.py:127-178, qwen36_router.py:96) and the 8-bit products
+ * it is made of.
+ *
+ * ria_quant_fp8: activations to e4m3.  Each 128 values of a row share a scale
+ * s = the smallest power of two with |x| / s <= 448 for every finite x of them
+ * (1 if all are 0, 2^-126 at the least); out = e4m3(x / s), to nearest even.
+ * x / s is exact, so the bits do not depend on an arithmetic's rounding.
+ * Infinities and NaN become NaN and leave the others' scale alone.
+ * x [rows, cols] of x_dtype, cols a multiple of 128, 16-byte aligned, row
+ * stride a multiple of 8; out [rows, cols] contiguous, 16-byte aligned; scale
+ * [rows, cols / 128].
+ *
+ * ria_linear_fp8_x8: y = (x x_scale) (w scale_inv)^T with both operands in
+ * e4m3: x [m, k] with one scale per 128 values of a row (ria_quant_fp8's, or
+ * any), weight [n, k] with one per 128 x 128 block as in ria_linear_fp8; fp32
+ * accumulation, one rounding to y_dtype; with y_add, y (fp32) += the result.
+ * n a multiple of 16, k of 128 up to 32768; x and weight 16-byte aligned, x
+ * row stride a multiple of 16.
+ */
+int ria_quant_fp8(int64_t rows, int cols, const void* x, int x_dtype, int64_t x_row_stride, void* out, float* scale,
+                  void* stream);
+
+int ria_linear_fp8_x8(int m, int n, int k, const void* x, int64_t x_row_stride, const float* x_scale,
+                      int64_t x_scale_row_stride, const void* weight, const float* scale_inv, void* y, int y_dtype,
+                      int64_t y_row_stride, int y_add, void* stream);
+
+/* How ria_moe_route turns logits into scores, and scores into a group's rank. */
+enum ria_route_scoring { RIA_ROUTE_SOFTMAX = 0, RIA_ROUTE_SIGMOID = 1 };
+enum ria_route_group_score { RIA_ROUTE_GROUP_MAX = 0, RIA_ROUTE_GROUP_TOP2 = 1 };
+
+/*
+ * Routing: each token's top_k experts and their weights from router logits
+ * (qwen36_router.py:96 `route`, which is softmax, top-k, renormalised).
+ *   score   softmax over the experts, or the sigmoid of each logit
+ *   choice  score + bias (bias f32 [experts] or NULL: the logits are compared)
+ *   groups  the experts split into num_groups equal runs; only the top_groups
+ *           of the best group score stay eligible (the best choice of a group,
+ *           or the sum of its best two)
+ *   ids     the top_k eligible experts of the largest choice, largest first;
+ *           equal ones (of groups too) go to the lowest index
+ *   weights their scores, divided by the chosen scores' sum if renormalize,
+ *           times scale
+ * Choices are compared in 64 bits.  An expert whose logit or bias is -inf is
+ * never chosen: a slot left over has id -1 and weight 0.  NaN ranks above every
+ * number, so it shows in the weights.  With shared_expert the logits have one
+ * column more, the gate of an expert that every token visits: slot top_k gets
+ * id `experts` and weight sigmoid(gate) (-1 and 0 where the gate is -inf).
+ * experts <= 1024, top_k <= 32, num_groups <= 64.
+ * logits [tokens, experts (+ 1)]; weights f32, ids i32 [tokens, top_k (+ 1)];
+ * row strides in elements.
+ */
+int ria_moe_route(int tokens, int experts, int top_k, const void* logits, int logits_dtype, int64_t logits_row_stride,
+                  int scoring, const float* bias, int num_groups, int top_groups, int group_score, int renormalize,
+                  float scale, int shared_expert, float* weights, int64_t weights_row_stride, int32_t* ids,
+                  int64_t ids_row_stride, void* stream);
+
+/*
+ * The chosen experts' gated MLPs, summed with the router's weights:
+ *
+ *   (g | u) = W13[e] Q(x_t),   out_t = sum_j weights[t, j] W2[e] Q(SiLU(g) u),   e = ids[t, j]
+ *
+ * with Q as ria_quant_fp8 and both products as ria_linear_fp8_x8.  Each slot's
+ * term is rounded to out_dtype, the sum is fp32, rounded once more; with
+ * accumulate, out (fp32) += it.  Slots whose id is outside [0, experts) add
+ * nothing (a token without any gets 0); an expert may come twice in a row.
+ *   x     [tokens, hidden] of x_dtype, 16-byte aligned, row stride a multiple of 8
+ *   w13   [experts, 2 inter, hidden] e4m3, gate rows first; w13_scale_inv f32
+ *         [experts, 2 inter / 128, hidden / 128]
+ *   w2    [experts, hidden, inter] e4m3; w2_scale_inv [experts, hidden / 128, inter / 128]
+ *   workspace  ria_moe_experts_workspace_bytes() bytes (-1: sizes refused),
+ *         256-byte aligned, of this call alone until it is done
+ * hidden and inter multiples of 128 up to 32768, experts <= 1024.
+ */
+typedef struct ria_moe_experts_desc {
+  int tokens, top_k, experts, hidden, inter;
+  const void* x;
+  int x_dtype;
+  int64_t x_row_stride;
+  const int32_t* ids;
+  int64_t ids_row_stride;
+  const float* weights;
+  int64_t weights_row_stride;
+  const void* w13;
+  const float* w13_scale_inv;
+  const void* w2;
+  const float* w2_scale_inv;
+  void* out;
+  int out_dtype;
+  int64_t out_row_stride;
+  int accumulate;
+  void* workspace;
+  int64_t workspace_bytes;
+} ria_moe_experts_desc;
+
+int64_t ria_moe_experts_workspace_bytes(int tokens, int top_k, int experts, int hidden, int inter, int out_dtype);
+int ria_moe_experts(const ria_moe_experts_desc* desc, void* stream);
 
 /*
  * Sequence snapshots: one row's DeltaNet states, conv ring and KV pages as a

@@ -1,0 +1,111 @@
+// Activations quantised to e4m3 and their products with block-FP8 weights.
+//
+//   quant_fp8_kernel   x [rows, cols] -> e4m3 values and one power-of-two
+//                      scale per 128 values of a row.
+//   x8_tile_kernel     y = (x8 xs) (w8 ws)^T (x8_tile.h).
+//
+// The block-FP8 checkpoints whose weights linear_fp8.hip dequantises to fp16
+// name this as the way to run them: activations in e4m3, a scale for each
+// 128 values of a row, found as they come.  The reference multiplies in fp16
+// (qwen36_attention_cache.py:232-247), which linear_fp8.hip reproduces; here
+// both operands stay in 8 bits and the matrix cores run at twice the rate.
+#include "x8_tile.h"
+
+namespace ria {
+
+// One thread per 8 values, 16 threads per block of 128.
+template <int XT>
+__global__ __launch_bounds__(256) void quant_fp8_kernel(int64_t units, int per_row, const void* x, int64_t x_stride,
+                                                        uint8_t* out, float* scale) {
+  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (u >= units) return;  // whole groups of 16 threads
+  const int64_t r = u / per_row;
+  const int c = static_cast<int>(u - r * per_row) * 8;
+  float v[8];
+  load_act8<XT>(x, r * x_stride + c, v);
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(v[i]));
+  const uint32_t e = x8_scale_exp(row16_max(top));
+  const float inv = x8_inverse(e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = x8_value(v[i], inv);
+  *reinterpret_cast<u32x2*>(out + u * 8) = u32x2{pack_x8(v[0], v[1], v[2], v[3]), pack_x8(v[4], v[5], v[6], v[7])};
+  if ((threadIdx.x & 15) == 0) scale[u / 16] = x8_scale(e);
+}
+
+bool x8_dtype_ok(int dt) { return dt == RIA_DT_BF16 || dt == RIA_DT_F16 || dt == RIA_DT_F32; }
+
+int launch_quant_fp8(const char* who, int64_t rows, int cols, const void* x, int x_dtype, int64_t x_row_stride,
+                     void* out, float* scale, hipStream_t st) {
+  const int64_t units = rows * (cols / 8), blocks = (units + 255) / 256;
+  if (blocks > 0x7fffffff) return set_error(RIA_ERR_INVALID, "%s: too many values", who);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  uint8_t* o = static_cast<uint8_t*>(out);
+  if (x_dtype == RIA_DT_BF16)
+    hipLaunchKernelGGL((quant_fp8_kernel<RIA_DT_BF16>), grid, dim3(256), 0, st, units, cols / 8, x, x_row_stride, o, scale);
+  else if (x_dtype == RIA_DT_F16)
+    hipLaunchKernelGGL((quant_fp8_kernel<RIA_DT_F16>), grid, dim3(256), 0, st, units, cols / 8, x, x_row_stride, o, scale);
+  else
+    hipLaunchKernelGGL((quant_fp8_kernel<RIA_DT_F32>), grid, dim3(256), 0, st, units, cols / 8, x, x_row_stride, o, scale);
+  return check_launch(who);
+}
+
+
+}  // namespace ria
+
+using namespace ria;
+
+extern "C" int ria_quant_fp8(int64_t rows, int cols, const void* x, int x_dtype, int64_t x_row_stride, void* out,
+                             float* scale, void* stream) {
+  const char* who = "ria_quant_fp8";
+  if (rows < 0 || cols <= 0 || cols % kX8Block)
+    return set_error(RIA_ERR_INVALID, "%s: cols must be a positive multiple of %d (got %d)", who, kX8Block, cols);
+  if (!x8_dtype_ok(x_dtype)) return set_error(RIA_ERR_INVALID, "%s: unknown dtype code", who);
+  if (rows == 0) return RIA_OK;
+  if (!x || !out || !scale) return set_error(RIA_ERR_INVALID, "%s: null pointer", who);
+  if (x_row_stride < cols || x_row_stride % 8 || reinterpret_cast<uintptr_t>(x) % 16)
+    return set_error(RIA_ERR_INVALID, "%s: x must be 16-byte aligned with a row stride of at least cols, a multiple of 8", who);
+  if (reinterpret_cast<uintptr_t>(out) % 16) return set_error(RIA_ERR_INVALID, "%s: out must be 16-byte aligned", who);
+  return launch_quant_fp8(who, rows, cols, x, x_dtype, x_row_stride, out, scale, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int ria_linear_fp8_x8(int m, int n, int k, const void* x, int64_t x_row_stride, const float* x_scale,
+                                 int64_t x_scale_row_stride, const void* weight, const float* scale_inv, void* y,
+                                 int y_dtype, int64_t y_row_stride, int y_add, void* stream) {
+  const char* who = "ria_linear_fp8_x8";
+  if (m < 0 || n <= 0 || n % 16) return set_error(RIA_ERR_INVALID, "%s: N must be a positive multiple of 16 (got %d)", who, n);
+  if (k <= 0 || k % kX8Block || k > 32768)
+    return set_error(RIA_ERR_INVALID, "%s: K must be a multiple of %d up to 32768 (got %d)", who, kX8Block, k);
+  if (!x8_dtype_ok(y_dtype)) return set_error(RIA_ERR_INVALID, "%s: unknown dtype code", who);
+  if (y_add && y_dtype != RIA_DT_F32) return set_error(RIA_ERR_INVALID, "%s: y_add needs an fp32 y", who);
+  if (m == 0) return RIA_OK;
+  if (!x || !x_scale || !weight || !scale_inv || !y) return set_error(RIA_ERR_INVALID, "%s: null pointer", who);
+  if (x_row_stride < k || x_row_stride % 16 || reinterpret_cast<uintptr_t>(x) % 16)
+    return set_error(RIA_ERR_INVALID, "%s: x must be 16-byte aligned with a row stride of at least K, a multiple of 16", who);
+  if (x_scale_row_stride < k / kX8Block) return set_error(RIA_ERR_INVALID, "%s: x_scale row stride too small", who);
+  if (y_row_stride < n) return set_error(RIA_ERR_INVALID, "%s: y row stride too small", who);
+  if (reinterpret_cast<uintptr_t>(weight) % 16) return set_error(RIA_ERR_INVALID, "%s: weight must be 16-byte aligned", who);
+  X8Args a{};
+  a.x = static_cast<const uint8_t*>(x);
+  a.x_stride = x_row_stride;
+  a.xs = x_scale;
+  a.xs_stride = x_scale_row_stride;
+  a.w = static_cast<const uint8_t*>(weight);
+  a.ws = scale_inv;
+  a.m = m;
+  a.n = n;
+  a.k = k;
+  a.y = y;
+  a.y_stride = y_row_stride;
+  a.y_dtype = y_dtype;
+  a.y_add = y_add;
+  a.vec = reinterpret_cast<uintptr_t>(y) % 16 == 0 && y_row_stride % 8 == 0;
+  if ((m + 127) / 128 > 65535) return set_error(RIA_ERR_INVALID, "%s: too many rows", who);
+  const dim3 grid((n + 127) / 128, (m + 127) / 128);
+  if (y_dtype == RIA_DT_F32)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, true>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  else
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, false>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  return check_launch(who);
+}

@@ -15,7 +15,7 @@ from pathlib import Path
 
 LIB_ENV = "RIA_HIP_LIB"
 DEFAULT_LIB = Path(__file__).resolve().parent / "_lib" / "libria_hip.so"
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 RIA_DT_BF16 = 0
 RIA_DT_F16 = 1
@@ -33,6 +33,10 @@ RIA_CONV_RING = 1
 RIA_CONV_WINDOW = 2
 RIA_QK_RAW = 0
 RIA_QK_NORMALIZED = 1
+RIA_ROUTE_SOFTMAX = 0
+RIA_ROUTE_SIGMOID = 1
+RIA_ROUTE_GROUP_MAX = 0
+RIA_ROUTE_GROUP_TOP2 = 1
 
 _c_int = ctypes.c_int
 _c_i32 = ctypes.c_int32
@@ -113,6 +117,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "ria_linear_fp8": (_c_int, [_c_int, _c_int, _c_int, _vp, _c_int, _c_i64, _vp, _vp, _vp, _c_int, _c_i64, _vp]),
     "ria_linear_fp8_group": (_c_int, [_c_int, _c_int, _vp, _c_int, _c_i64, _c_int, _vp, _vp]),
     "ria_linear_fp8_group_normed": (_c_int, [_c_int, _c_int, _vp, _c_i64, _vp, _c_f32, _c_int, _c_int, _vp, _vp]),
+    "ria_quant_fp8": (_c_int, [_c_i64, _c_int, _vp, _c_int, _c_i64, _vp, _vp, _vp]),
+    "ria_linear_fp8_x8": (
+        _c_int,
+        [_c_int, _c_int, _c_int, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _c_int, _c_i64, _c_int, _vp],
+    ),
+    "ria_moe_route": (
+        _c_int,
+        [_c_int, _c_int, _c_int, _vp, _c_int, _c_i64, _c_int, _vp, _c_int, _c_int, _c_int, _c_int, _c_f32, _c_int,
+         _vp, _c_i64, _vp, _c_i64, _vp],
+    ),
+    "ria_moe_experts_workspace_bytes": (_c_i64, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "ria_moe_experts": (_c_int, [_vp, _vp]),
     "ria_seq_state_bytes": (_c_i64, [_c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
     "ria_seq_state_save": (
         _c_int,
@@ -193,6 +209,15 @@ class Fp8Proj(ctypes.Structure):
     """struct ria_fp8_proj: one projection of a ria_linear_fp8_group call."""
     _fields_ = [("weight", _vp), ("scale_inv", _vp), ("y", _vp), ("y_row_stride", _c_i64), ("n", _c_int),
                 ("y_dtype", _c_int), ("y_add", _c_int)]
+
+
+class MoeExpertsDesc(ctypes.Structure):
+    """struct ria_moe_experts_desc: one ria_moe_experts call."""
+    _fields_ = [("tokens", _c_int), ("top_k", _c_int), ("experts", _c_int), ("hidden", _c_int), ("inter", _c_int),
+                ("x", _vp), ("x_dtype", _c_int), ("x_row_stride", _c_i64), ("ids", _vp), ("ids_row_stride", _c_i64),
+                ("weights", _vp), ("weights_row_stride", _c_i64), ("w13", _vp), ("w13_scale_inv", _vp), ("w2", _vp),
+                ("w2_scale_inv", _vp), ("out", _vp), ("out_dtype", _c_int), ("out_row_stride", _c_i64),
+                ("accumulate", _c_int), ("workspace", _vp), ("workspace_bytes", _c_i64)]
 
 
 LINEAR_GROUP_MAX = 4  # projections per ria_linear_fp8_group call

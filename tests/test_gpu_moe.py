@@ -1,0 +1,356 @@
+"""GPU parity: expert routing, e4m3 activations, FP8 x FP8 products and the experts' MLPs.
+
+Every operator is compared with its definition in 64 bits, computed here on the
+CPU from the same inputs.  Tolerances count roundings: half a step of the
+output's type (eps / 2 relative), and for fp32 sums of n terms the error of
+their order, n * 2^-24 of the sum of the terms' magnitudes at most.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from conftest import announce
+from router_ia import kernels as K
+
+pytestmark = pytest.mark.gpu
+
+BLOCK = 128
+E4M3 = torch.float8_e4m3fn
+
+
+def half_step(dtype: torch.dtype) -> float:
+    return torch.finfo(dtype).eps / 2
+
+
+# ----------------------------------------------------------------------------- definitions in 64 bits
+def quant64(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(e4m3 values as float64, scales): the smallest power of two s with |x| / s <= 448 for the finite x of a block."""
+    b = x.double().unflatten(-1, (-1, BLOCK))
+    top = torch.where(torch.isfinite(b), b, 0.0).abs().amax(-1)
+    s = torch.exp2(torch.ceil(torch.log2(top / 448.0)).clamp(min=-126.0))
+    s = torch.where(top > 0, s, 1.0)
+    v = b / s[..., None]
+    step = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -20))).clamp(min=-6.0) - 3.0)
+    q = torch.where(torch.isfinite(v), torch.round(v / step) * step, math.nan)
+    return q.flatten(-2), s
+
+
+def widen(w: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
+    """Block-scaled e4m3 weights [.., n, k] in 64 bits."""
+    n, k = w.shape[-2:]
+    return w.double() * s.double().repeat_interleave(BLOCK, -2)[..., :n, :].repeat_interleave(BLOCK, -1)[..., :k]
+
+
+def rows64(q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
+    return (q.double().unflatten(-1, (-1, BLOCK)) * s.double()[..., None]).flatten(-2)
+
+
+def route64(logits, k, scoring="softmax", bias=None, num_groups=1, top_groups=1, group_score="top2",
+            renormalize=True, scale=1.0, shared_expert=False):
+    e = logits.shape[1] - int(shared_expert)
+    out_w, out_i = [], []
+    for row in logits.double():
+        x = [float(v) for v in row[:e]]
+        if scoring == "softmax":
+            m = max(x)
+            p = [math.exp(v - m) if v > -math.inf else 0.0 for v in x]
+            z = sum(p)
+            p = [v / z if z else 0.0 for v in p]
+        else:
+            p = [1.0 / (1.0 + math.exp(-v)) if v > -700 else 0.0 for v in x]
+        c = [a + (float(bias[i]) if bias is not None else 0.0) if x[i] > -math.inf else -math.inf
+             for i, a in enumerate(p)]
+        per = e // num_groups
+        rank = []
+        for g in range(num_groups):
+            best = sorted(c[g * per:(g + 1) * per], reverse=True)
+            rank.append(best[0] if group_score == "max" or per == 1 else best[0] + best[1])
+        keep = sorted(range(num_groups), key=lambda g: (-rank[g], g))[:top_groups]
+        order = sorted((i for i in range(e) if i // per in keep and c[i] > -math.inf), key=lambda i: (-c[i], i))[:k]
+        w = [p[i] for i in order]
+        if renormalize and sum(w):
+            w = [v / sum(w) for v in w]
+        w = [v * scale for v in w] + [0.0] * (k - len(order))
+        order = order + [-1] * (k - len(order))
+        if shared_expert:
+            gate = float(row[e])
+            w.append(1.0 / (1.0 + math.exp(-gate)) if gate > -700 else 0.0)
+            order.append(e if gate > -math.inf else -1)
+        out_w.append(w)
+        out_i.append(order)
+    return torch.tensor(out_w, dtype=torch.float64), torch.tensor(out_i, dtype=torch.int32)
+
+
+def experts64(x, ids, weights, w13, s13, w2, s2):
+    """The sum over the slots, and the sum of the slots' magnitudes (for the tolerance)."""
+    e, i = w13.shape[0], w2.shape[2]
+    xq = rows64(*quant64(x))
+    out = torch.zeros(x.shape, dtype=torch.float64)
+    mag = torch.zeros_like(out)
+    for j in range(e):
+        rows, slot = torch.nonzero(ids == j, as_tuple=True)
+        if rows.numel() == 0:
+            continue
+        z = xq[rows] @ widen(w13[j], s13[j]).T
+        a = z[:, :i] * torch.sigmoid(z[:, :i]) * z[:, i:]
+        term = rows64(*quant64(a)) @ widen(w2[j], s2[j]).T * weights[rows, slot].double()[:, None]
+        out.index_add_(0, rows, term)
+        mag.index_add_(0, rows, term.abs())
+    return out, mag
+
+
+# ----------------------------------------------------------------------------- inputs
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def e4m3_weight(seed, *shape):
+    g = gen(seed)
+    w = (torch.randn(shape, generator=g) * 100.0).clamp(-448, 448).to(E4M3)
+    blocks = shape[:-2] + ((shape[-2] + BLOCK - 1) // BLOCK, shape[-1] // BLOCK)
+    return w, 2e-4 * (0.5 + torch.rand(blocks, generator=g))
+
+
+# ----------------------------------------------------------------------------- quantisation
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,k", [(1, 128), (3, 384), (129, 2048), (517, 896)])
+def test_quant_matches_definition_bit_for_bit(gpu, m, k, dtype):
+    announce(f"quant_fp8: {m} x {k} {dtype}")
+    x = torch.randn((m, k + 8), generator=gen(m + k)) * torch.exp(3 * torch.randn((m, 1), generator=gen(k)))
+    x = x.to(dtype)
+    q, s = K.quant_fp8(x.to(gpu)[:, :k])  # rows of a wider buffer
+    x = x[:, :k]
+    want_q, want_s = quant64(x)
+    assert torch.equal(s.cpu().double(), want_s)
+    assert torch.equal(q.cpu().double(), want_q)
+
+
+def test_quant_edges(gpu):
+    """Zero blocks, the largest and smallest fp32, exact 448 multiples, ties, infinities and NaN."""
+    announce("quant_fp8: edge values")
+    x = torch.zeros((10, 128))
+    x[1, 0] = 448.0                      # scale 1 exactly
+    x[2, 0] = 448.0000305                # the next fp32: scale 2
+    x[3] = torch.linspace(-3e38, 3e38, 128)
+    x[4, :4] = torch.tensor([1e-45, 2e-45, -1e-44, 0.0])  # smallest fp32 values: scale 2^-126
+    x[5, :8] = torch.tensor([448.0, 17.0, 19.0, -17.0, 2.0 ** -10, 3 * 2.0 ** -10, 2.0 ** -9, -2.0 ** -10])  # ties
+    x[6, :4] = torch.tensor([math.inf, -math.inf, 3.0, math.nan])
+    x[7] = math.nan
+    x[8, 5] = -math.inf
+    x[9] = torch.randn(128, generator=gen(9)) * 1e-30
+    q, s = K.quant_fp8(x.to(gpu))
+    want_q, want_s = quant64(x)
+    assert torch.equal(s.cpu().double(), want_s)
+    torch.testing.assert_close(q.cpu().double(), want_q, rtol=0, atol=0, equal_nan=True)
+
+
+# ----------------------------------------------------------------------------- dense product
+LINEAR = [  # (m, n, k)
+    (1, 16, 128), (1, 8192, 2048), (2, 48, 256), (5, 400, 1152), (16, 512, 2048), (17, 2048, 4096), (33, 144, 128),
+    (64, 1040, 640), (100, 2048, 512), (129, 272, 2048), (200, 1536, 384), (300, 2048, 4096), (513, 784, 896),
+    (1025, 4112, 256),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", LINEAR)
+def test_linear_x8_matches_definition(gpu, m, n, k, dtype):
+    announce(f"linear_fp8_x8: {m} x {n} x {k} -> {dtype}")
+    x = torch.randn((m, k), generator=gen(m)) * (1 + 9 * (torch.rand((k,), generator=gen(k)) < 0.02))
+    q, s = quant64(x)
+    s = s * (0.5 + torch.rand(s.shape, generator=gen(n)))  # any fp32 scales are taken
+    q, s = q.to(E4M3), s.float()
+    w, ws = e4m3_weight(n + k, n, k)
+    # rows of wider buffers
+    qd = torch.nn.functional.pad(q.view(torch.uint8), (0, 16)).to(gpu)[:, :k].view(E4M3)
+    sd = torch.nn.functional.pad(s, (0, 3)).to(gpu)[:, : k // BLOCK]
+    y = K.linear_fp8_x8(qd, sd, w.to(gpu), ws.to(gpu), out_dtype=dtype)
+    xw, ww = rows64(q, s), widen(w, ws)
+    want, mag = xw @ ww.T, xw.abs() @ ww.abs().T
+    # k products summed in fp32 in some order, two scalings per block, and the rounding of the result
+    tol = half_step(dtype) * want.abs() + (k + 4) * 2.0 ** -24 * mag
+    if dtype != torch.float32:
+        # 16-bit results may come from the matrix cores' e4m3 products, which cut each product of a group of 16
+        # 13 bits below the group's largest: 16 * 2^-13 of the largest, itself at most the group's magnitudes
+        tol = tol + 2.0 ** -9 * mag
+    err = (y.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), f"{(err / tol).max().item():.3g} of the tolerance"
+
+
+def test_linear_x8_accumulate_strided_out_and_stream(gpu):
+    announce("linear_fp8_x8: accumulate into a strided fp32 out, another stream")
+    m, n, k = 37, 272, 256
+    q, s = quant64(torch.randn((m, k), generator=gen(1)))
+    w, ws = e4m3_weight(2, n, k)
+    base = torch.randn((m, n + 12), generator=gen(3))
+    out = base.to(gpu)
+    args = q.to(E4M3).to(gpu), s.float().to(gpu), w.to(gpu), ws.to(gpu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K.linear_fp8_x8(*args, out=out[:, 5:5 + n], accumulate=True)
+    side.synchronize()
+    want = base.double()
+    want[:, 5:5 + n] += rows64(q, s) @ widen(w, ws).T
+    mag = rows64(q, s).abs() @ widen(w, ws).abs().T
+    got = out.cpu().double()
+    assert torch.equal(got[:, :5], base[:, :5].double()) and torch.equal(got[:, 5 + n:], base[:, 5 + n:].double())
+    tol = 2.0 ** -24 * want[:, 5:5 + n].abs() + (k + 4) * 2.0 ** -24 * mag
+    assert bool(((got - want)[:, 5:5 + n].abs() <= tol).all())
+
+
+def test_linear_x8_nan_stays_in_its_row(gpu):
+    announce("linear_fp8_x8: a NaN value shows in its row alone")
+    x = torch.randn((20, 256), generator=gen(1))
+    x[7, 130] = math.nan
+    q, s = K.quant_fp8(x.to(gpu))
+    w, ws = e4m3_weight(2, 64, 256)
+    y = K.linear_fp8_x8(q, s, w.to(gpu), ws.to(gpu)).cpu()
+    bad = torch.isnan(y)
+    assert bool(bad[7].all()) and not bool(bad[torch.arange(20) != 7].any())
+
+
+# ----------------------------------------------------------------------------- routing
+ROUTES = [
+    dict(t=1, e=256, k=8),
+    dict(t=5, e=8, k=8),
+    dict(t=67, e=60, k=4, renormalize=False),
+    dict(t=33, e=100, k=7, scoring="sigmoid", scale=2.5),
+    dict(t=40, e=256, k=8, scoring="sigmoid", bias=True, num_groups=8, top_groups=4, shared_expert=True),
+    dict(t=30, e=160, k=6, num_groups=8, top_groups=3, group_score="max"),
+    dict(t=30, e=160, k=6, num_groups=8, top_groups=3, group_score="top2"),
+    dict(t=30, e=24, k=3, num_groups=24, top_groups=5, bias=True),
+    dict(t=30, e=512, k=16, bias=True, scale=0.5, renormalize=False),
+    dict(t=9, e=1000, k=32, num_groups=4, top_groups=2, bias=True, shared_expert=True),
+    dict(t=9, e=1, k=1),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("case", ROUTES, ids=lambda c: f"t{c['t']}_e{c['e']}_k{c['k']}")
+@pytest.mark.parametrize("masked", [False, True])
+def test_route_matches_definition(gpu, case, dtype, masked):
+    c = dict(case)
+    t, e, k = c.pop("t"), c.pop("e"), c.pop("k")
+    announce(f"moe_route: {t} tokens, {k} of {e} {dtype} {c} masked {masked}")
+    cols = e + int(c.get("shared_expert", False))
+    x = (torch.randn((t, cols), generator=gen(e + t)) * 1.5).to(dtype)
+    if masked:
+        x.masked_fill_(torch.rand((t, cols), generator=gen(e)) < 0.6, -math.inf)
+        x[0] = -math.inf
+    if c.pop("bias", False):
+        c["bias"] = torch.randn((e,), generator=gen(3)) * 0.2
+    want_w, want_i = route64(x, k, **c)
+    if "bias" in c:
+        c["bias"] = c["bias"].to(gpu)
+    wide = torch.nn.functional.pad(x, (0, 5)).to(gpu)[:, :cols]
+    w, i = K.moe_route(wide, k, **c)
+    assert torch.equal(i.cpu(), want_i)
+    # computed in 64 bits (or fp32 with a handful of roundings), rounded once to fp32
+    torch.testing.assert_close(w.cpu().double(), want_w, rtol=16 * 2.0 ** -24, atol=1e-38)
+
+
+def test_route_ties_go_to_the_lowest_index(gpu):
+    announce("moe_route: ties")
+    x = torch.zeros((3, 130))
+    x[1, 100:] = 1.0
+    x[2, ::2] = -0.0
+    w, i = K.moe_route(x.to(gpu), 5)
+    assert i.cpu().tolist() == [[0, 1, 2, 3, 4], [100, 101, 102, 103, 104], [0, 1, 2, 3, 4]]
+    torch.testing.assert_close(w.cpu(), torch.full((3, 5), 0.2), rtol=2.0 ** -23, atol=0)
+    _, i = K.moe_route(torch.zeros((1, 64), device=gpu), 3, scoring="sigmoid", num_groups=8, top_groups=2,
+                       bias=torch.zeros(64, device=gpu))
+    assert i.cpu().tolist() == [[0, 1, 2]]
+
+
+def test_route_near_ties_follow_64_bits(gpu):
+    """A bias that brings unlike scores within 1e-9 of each other: fp32 could not order them."""
+    announce("moe_route: scores and biases that nearly cancel")
+    g = gen(5)
+    x = torch.randn((64, 128), generator=g)
+    p = torch.sigmoid(x[0].double())
+    bias = (1.0 - p).float()  # token 0: every choice within fp32 roundings of 1
+    want_w, want_i = route64(x, 8, scoring="sigmoid", bias=bias)
+    w, i = K.moe_route(x.to(gpu), 8, scoring="sigmoid", bias=bias.to(gpu))
+    assert torch.equal(i.cpu(), want_i)
+    torch.testing.assert_close(w.cpu().double(), want_w, rtol=16 * 2.0 ** -24, atol=0)
+
+
+def test_route_extreme_logits(gpu):
+    announce("moe_route: saturated, infinite and NaN logits")
+    x = torch.zeros((6, 16))
+    x[0] = -200.0
+    x[0, 3] = -190.0
+    x[1] = torch.linspace(50.0, 80.0, 16)      # sigmoids that round to 1: the logits rank
+    x[2, 2], x[2, 9] = math.nan, 5.0
+    x[3, 4] = math.inf
+    x[4] = -3e38
+    x[5] = 3e38
+    w, i = K.moe_route(x.to(gpu), 2, scoring="softmax")
+    w, i = w.cpu(), i.cpu()
+    assert i[0].tolist() == [3, 0] and i[1].tolist() == [15, 14] and i[4].tolist() == [0, 1] and i[5].tolist() == [0, 1]
+    assert i[2].tolist() == [2, 9] and bool(torch.isnan(w[2]).all())
+    assert i[3, 0] == 4 and bool(torch.isnan(w[3]).any())
+    torch.testing.assert_close(w[0], torch.tensor([1.0, math.exp(-10.0)]) / (1 + math.exp(-10.0)), rtol=1e-6, atol=0)
+    w, i = K.moe_route(x.to(gpu), 2, scoring="sigmoid")
+    assert i[1].tolist() == [15, 14] and i[0].tolist() == [3, 0]
+    torch.testing.assert_close(w[0].cpu(), torch.tensor([1.0, math.exp(-10.0)]) / (1 + math.exp(-10.0)), rtol=1e-6, atol=0)
+
+
+# ----------------------------------------------------------------------------- experts
+EXPERTS = [  # (tokens, experts, top_k, hidden, inter)
+    (1, 8, 2, 256, 128), (1, 16, 8, 2048, 512), (2, 4, 1, 128, 128), (3, 5, 5, 384, 256), (7, 16, 3, 512, 640),
+    (17, 3, 2, 256, 128), (40, 33, 4, 256, 384), (130, 6, 2, 640, 256), (200, 2, 2, 256, 128), (300, 40, 6, 512, 128),
+    (700, 3, 2, 256, 256),
+]
+
+
+def expert_inputs(t, e, k, h, i, dtype, seed):
+    g = gen(seed)
+    x = torch.randn((t, h), generator=g).to(dtype)
+    ids = torch.stack([torch.randperm(e, generator=g)[:k] for _ in range(t)]).to(torch.int32)
+    weights = torch.rand((t, k), generator=g) + 0.05
+    w13, s13 = e4m3_weight(seed + 1, e, 2 * i, h)
+    w2, s2 = e4m3_weight(seed + 2, e, h, i)
+    return x, ids, weights, w13, s13, w2, s2
+
+
+def expert_tolerance(out, mag, k, dtype, slack):
+    """Roundings of the slots' terms and of the sum to out's type, and the fp32 sums' own.
+
+    The hidden values are e4m3: where an fp32 sum of another order lies on the
+    other side of a rounding border, one value moves by a step, 2^-3 of itself
+    at most.  `slack` bounds what such moves add, relative to the row's size.
+    """
+    size = out.abs().amax(-1, keepdim=True)
+    return half_step(dtype) * (out.abs() + mag) + 1e-5 * mag + slack * size
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t,e,k,h,i", EXPERTS)
+def test_experts_match_definition(gpu, t, e, k, h, i, dtype):
+    announce(f"moe_experts: {t} tokens, {k} of {e}, {h} x {i} {dtype}")
+    a = expert_inputs(t, e, k, h, i, dtype, t + h)
+    if t > 2:
+        a[1][1] = -1              # a token without experts
+        a[1][2, 0] = e            # ids past the experts add nothing
+    want, mag = experts64(*a)
+    out = K.moe_experts(*(v.to(gpu) for v in a)).cpu().double()
+    assert out.shape == want.shape
+    if t > 2:
+        assert not bool(out[1].any())
+    # one value of `i` moved by 2^-3 of itself changes a term by 2^-3 / sqrt(i) of its size, typically;
+    # the largest values are 4 sigma, and two may move in a row
+    err, tol = (out - want).abs(), expert_tolerance(want, mag, k, dtype, 0.125 * 4 * 2 / math.sqrt(i))
+    assert bool((err <= tol).all()), f"{(err / tol).max().item():.3g} of the tolerance"
+    if dtype != torch.float32:
+        return
+    # with an fp32 out every sum is in fp32, and such moves are rare: two fp32 sums of one value differ by some 2^-22 of it, its borders lie 2^-3 apart, so one
+    # of 2^19 / (4 sizes of safety) values moves; every other row lies within the roundings alone
+    tight = expert_tolerance(want, mag, k, dtype, 0.0)
+    moved = int((err > tight).any(-1).sum())
+    assert moved <= 1 + math.ceil(t * k * i * 2.0 ** -17), f"{moved} of {t} rows"
