@@ -101,11 +101,16 @@ extern "C" int ria_linear_fp8_x8(int m, int n, int k, const void* x, int64_t x_r
   a.y_dtype = y_dtype;
   a.y_add = y_add;
   a.vec = reinterpret_cast<uintptr_t>(y) % 16 == 0 && y_row_stride % 8 == 0;
-  if ((m + 127) / 128 > 65535) return set_error(RIA_ERR_INVALID, "%s: too many rows", who);
-  const dim3 grid((n + 127) / 128, (m + 127) / 128);
+  if (x_row_stride > (1 << 23)) return set_error(RIA_ERR_INVALID, "%s: x row stride over 8 MiB", who);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t t256 = (int64_t)((m + 255) / 256) * ((n + 255) / 256), t128 = (int64_t)((m + 127) / 128) * ((n + 127) / 128);
+  if (t128 > 0x7ffffff0) return set_error(RIA_ERR_INVALID, "%s: too many rows", who);
+  const dim3 g256(static_cast<unsigned>((t256 + 7) / 8 * 8)), g128(static_cast<unsigned>((t128 + 7) / 8 * 8));
   if (y_dtype == RIA_DT_F32)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, true>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, true>), g128, dim3(256), 0, st, a);
+  else if (t256 >= 256)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 4, 2, 2, 4, false>), g256, dim3(512), 0, st, a);
   else
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, false>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, false>), g128, dim3(256), 0, st, a);
   return check_launch(who);
 }

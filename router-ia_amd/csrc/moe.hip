@@ -326,6 +326,7 @@ static const char* moe_sizes_error(int64_t tokens, int top_k, int experts, int h
   if (hidden <= 0 || hidden % kX8Block || hidden > 32768) return "hidden must be a multiple of 128 up to 32768";
   if (inter <= 0 || inter % kX8Block || inter > 32768) return "inter must be a multiple of 128 up to 32768";
   if (tokens * top_k >= (int64_t(1) << 30)) return "too many (token, slot) pairs";
+  if (tokens * hidden >= (int64_t(1) << 32)) return "too many tokens (their e4m3 copy takes 4 GiB or more)";
   return nullptr;
 }
 
@@ -402,7 +403,8 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
   X8Tile* tiles = static_cast<X8Tile*>(at(l.tiles));
   int32_t* ntiles = static_cast<int32_t*>(at(l.ntiles));
   const int64_t pairs = (int64_t)d->tokens * d->top_k, most = moe_tiles(pairs, d->experts);
-  if (most > 65535) return set_error(RIA_ERR_INVALID, "%s: too many (token, slot) pairs", who);
+  if (most * (std::max(d->hidden, d->inter) / 128) > 0x7ffffff0)
+    return set_error(RIA_ERR_INVALID, "%s: too many (token, slot) pairs", who);
   if (int rc = launch_quant_fp8(who, d->tokens, d->hidden, d->x, d->x_dtype, d->x_row_stride, at(l.x8),
                                 static_cast<float*>(at(l.xs)), st))
     return rc;
@@ -423,12 +425,13 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
   up.top_k = d->top_k;
   up.h8 = static_cast<uint8_t*>(at(l.h8));
   up.hs = static_cast<float*>(at(l.hs));
+  up.m = d->tokens;
   const bool wide = d->out_dtype == RIA_DT_F32;
-  const dim3 ugrid(d->inter / kX8Block, static_cast<unsigned>(most)), dgrid(d->hidden / 128, static_cast<unsigned>(most));
+  auto grid_of = [&](int feature_tiles) { return dim3(static_cast<unsigned>((most * feature_tiles + 7) / 8 * 8)); };
   if (wide)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true>), ugrid, dim3(256), 0, st, up);
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true>), grid_of(d->inter / 128), dim3(256), 0, st, up);
   else
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false>), ugrid, dim3(256), 0, st, up);
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false>), grid_of(d->inter / 128), dim3(256), 0, st, up);
   X8Args dn = up;
   dn.x = up.h8;
   dn.x_stride = d->inter;
@@ -445,9 +448,9 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
   dn.pair_w = d->weights;
   dn.pair_w_stride = d->weights_row_stride;
   if (wide)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, true>), dgrid, dim3(256), 0, st, dn);
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, true>), grid_of(d->hidden / 128), dim3(256), 0, st, dn);
   else
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, false>), dgrid, dim3(256), 0, st, dn);
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, false>), grid_of(d->hidden / 128), dim3(256), 0, st, dn);
   const CombineArgs c{at(l.slots), d->ids, d->ids_row_stride, d->tokens, d->top_k, d->experts, d->hidden, d->out,
                       d->out_row_stride, d->accumulate};
   const dim3 grid(static_cast<unsigned>(((int64_t)d->tokens * (d->hidden / 4) + 255) / 256));

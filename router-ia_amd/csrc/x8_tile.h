@@ -130,22 +130,55 @@ struct X8Args {
   float* hs;
 };
 
-// Four results of a row at element o.  a.vec: rows and base allow whole-vector stores.
-__device__ __forceinline__ void store_quad(const X8Args& a, int64_t o, float (&v)[4]) {
+// Direct copies into LDS (16 bytes a lane, lane l at d + 16 l) through a buffer
+// resource, so that a lane's part of the address is one 32-bit offset.  (Device
+// functions of their own: the host pass of a kernel template refuses the builtins.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t x8_rsrc(const uint8_t* p, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, static_cast<int>(static_cast<uint32_t>(bytes)),
+                                           kBufferWord3);
+}
+__device__ __forceinline__ void x8_copy(__amdgpu_buffer_rsrc_t r, uint8_t* d, uint32_t lane_offset, int offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, d, 16, lane_offset, offset, 0, 0);
+}
+
+// Eight results of a row at element o.  a.vec: rows and base allow whole-vector stores.
+__device__ __forceinline__ void store_eight(const X8Args& a, int64_t o, const float (&v)[8]) {
   if (a.y_add) {  // fp32
     float* yp = static_cast<float*>(a.y) + o;
+    if (a.vec) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) yp[i] = add_rn(yp[i], v[i]);
+      for (int h = 0; h < 2; ++h) {
+        f32x4 t = reinterpret_cast<f32x4*>(yp)[h];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = add_rn(t[i], v[4 * h + i]);
+        reinterpret_cast<f32x4*>(yp)[h] = t;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) yp[i] = add_rn(yp[i], v[i]);
+    }
   } else if (!a.vec) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store_act_dt(a.y, o + i, v[i], a.y_dtype);
+    for (int i = 0; i < 8; ++i) store_act_dt(a.y, o + i, v[i], a.y_dtype);
   } else if (a.y_dtype == RIA_DT_F32) {
-    store_act4<RIA_DT_F32>(a.y, o, v);
-  } else if (a.y_dtype == RIA_DT_F16) {
-    store_act4<RIA_DT_F16>(a.y, o, v);
+    f32x4* yp = reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + o);
+    yp[0] = f32x4{v[0], v[1], v[2], v[3]};
+    yp[1] = f32x4{v[4], v[5], v[6], v[7]};
   } else {
-    store_act4<RIA_DT_BF16>(a.y, o, v);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = a.y_dtype == RIA_DT_F16 ? Kv16<RIA_DT_F16>::pack2(v[2 * i], v[2 * i + 1])
+                                     : Kv16<RIA_DT_BF16>::pack2(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.y) + o) = u32x4{w[0], w[1], w[2], w[3]};
   }
+}
+
+// Workgroup b of a launch takes tile x8_order(b, total): the workgroups that
+// one XCD runs (b % 8) take consecutive tiles, whose operands meet in its L2.
+__device__ __forceinline__ int x8_order(int b, int total) {
+  const int per = (total + 7) / 8;
+  return b / 8 < per ? (b % 8) * per + b / 8 : total;
 }
 
 // A workgroup takes BN = 32 WF NF features x BM = 32 WT NT rows of x, a wave
@@ -153,7 +186,7 @@ __device__ __forceinline__ void store_quad(const X8Args& a, int64_t o, float (&v
 // row of x (lane % 32) and, of each 32 features, 8 q + 4 (lane / 32) + i.  Each
 // step stages one block of K, 128 bytes a row, in LDS by direct copies, chunk
 // c of row r at chunk c ^ ((r >> 1) & 7), so that the 16 lanes of a read's
-// phase meet all 64 banks.
+// phase meet all 64 banks; the next step's copies run beside the products.
 template <int MODE, int WF, int WT, int NF, int NT, bool WIDE>
 __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
   constexpr int NW = NF * NT;
@@ -161,70 +194,83 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
   constexpr int WL = BN / 8 / NW, XL = BM / 8 / NW;  // 1 KiB copies of a wave per step
   static_assert(WL * 8 * NW == BN && XL * 8 * NW == BM, "whole copies");
   static_assert(MODE != kX8Up || (BN == 256 && WF % 2 == 0), "one block of 128 gate and 128 up features");
-  constexpr int kHalf = (BN + BM) * kX8Block;  // bytes of a step
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kHalf];
+  constexpr int kStep = (BN + BM) * kX8Block;  // bytes of a step
+  constexpr int kPitch = 64 + 4;               // fp32 values of a row that a wave stages for its stores
+  constexpr int kStage = 32 * kPitch * 4;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kStep > NW * kStage ? 2 * kStep : NW * kStage];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wf = wave % NF, wt = wave / NF;
   const int l32 = lane & 31, half = lane >> 5;
 
-  int expert = 0, first = 0, rows = 0;
+  const int ntn = MODE == kX8Up ? a.n / 256 : (a.n + BN - 1) / BN;  // feature tiles
+  int expert = 0, first = 0, rows = 0, tn = 0;
   if constexpr (MODE == kX8Dense) {
-    first = blockIdx.y * BM;
+    const int ntm = (a.m + BM - 1) / BM;
+    const int at = x8_order(blockIdx.x, ntm * ntn);
+    if (at >= ntm * ntn) return;
+    // four row tiles by all feature tiles at a time
+    const int g0 = at / (4 * ntn) * 4, gs = min(4, ntm - g0), in = at - g0 * ntn;
+    first = (g0 + in % gs) * BM;
+    tn = in / gs;
     rows = min(BM, a.m - first);
   } else {
-    if (static_cast<int>(blockIdx.y) >= *a.ntiles) return;
-    const X8Tile t = a.tiles[blockIdx.y];
+    const int total = *a.ntiles * ntn;
+    const int at = x8_order(blockIdx.x, total);
+    if (at >= total) return;
+    const X8Tile t = a.tiles[at / ntn];
+    tn = at % ntn;
     expert = t.expert;
     first = t.first;
     rows = t.rows;
   }
-  const int n0 = blockIdx.x * BN;
+  const int n0 = tn * BN;
   const int kblocks = a.k / kX8Block;
   const int nblocks = (a.n + kX8Block - 1) / kX8Block;
   const uint8_t* w = a.w + (int64_t)expert * a.n * a.k;
   const float* ws = a.ws + (int64_t)expert * nblocks * kblocks;
 
-  // row of w behind tile row r: kX8Up takes 16 WF gate and 16 WF up rows for each wave
+  // Tile row r of the weights: kX8Up takes 16 WF gate and 16 WF up rows for
+  // each wave; features past n and rows past the last repeat the last one
+  // (computed, never stored).
   auto weight_row = [&](int r) {
     if constexpr (MODE == kX8Up) {
       const int g = r / (32 * WF), i = r % (32 * WF);
-      const int f = blockIdx.x * 128 + g * 16 * WF + i % (16 * WF);
-      return i < 16 * WF ? f : a.n / 2 + f;
+      return g * 16 * WF + i % (16 * WF) + (i < 16 * WF ? 0 : a.n / 2);
     } else {
-      return min(n0 + r, a.n - 1);  // features past n repeat the last one: computed, never stored
+      return min(r, a.n - 1 - n0);
     }
   };
-  auto x_row = [&](int r) -> int64_t {  // rows past the last likewise
+  auto x_row = [&](int r) -> int64_t {
     const int p = first + min(r, rows - 1);
     if constexpr (MODE == kX8Up)
       return a.order[p] / a.top_k;
     else
       return p;
   };
-  const uint8_t* wp[WL];
-  const uint8_t* xp[XL];
+  const int64_t x0 = MODE == kX8Up ? 0 : first;  // the resource starts at this row
+  const __amdgpu_buffer_rsrc_t wr =
+      MODE == kX8Up ? x8_rsrc(w + (int64_t)tn * 128 * a.k, (int64_t)(a.n - tn * 128) * a.k)
+                    : x8_rsrc(w + (int64_t)n0 * a.k, (int64_t)min(BN, a.n - n0) * a.k);
+  const __amdgpu_buffer_rsrc_t xr =
+      x8_rsrc(a.x + x0 * a.x_stride, MODE == kX8Up ? a.m * a.x_stride : (rows - 1) * a.x_stride + a.k);
+  uint32_t wo[WL], xo[XL];
 #pragma unroll
   for (int i = 0; i < WL; ++i) {
     const int r = (wave * WL + i) * 8 + (lane >> 3);
-    wp[i] = w + (int64_t)weight_row(r) * a.k + 16 * ((lane & 7) ^ ((r >> 1) & 7));
+    wo[i] = static_cast<uint32_t>(weight_row(r)) * a.k + 16 * ((lane & 7) ^ ((r >> 1) & 7));
   }
 #pragma unroll
   for (int i = 0; i < XL; ++i) {
     const int r = (wave * XL + i) * 8 + (lane >> 3);
-    xp[i] = a.x + x_row(r) * a.x_stride + 16 * ((lane & 7) ^ ((r >> 1) & 7));
+    xo[i] = static_cast<uint32_t>((x_row(r) - x0) * a.x_stride) + 16 * ((lane & 7) ^ ((r >> 1) & 7));
   }
-  auto issue = [&](int kb, int buf) {
-    uint8_t* d = lds + buf * kHalf;
+  auto issue = [&](int kb) __attribute__((always_inline)) {
+    uint8_t* d = lds + (kb & 1) * kStep;
 #pragma unroll
-    for (int i = 0; i < WL; ++i)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(wp[i] + kb * kX8Block),
-                                       (__attribute__((address_space(3))) void*)(d + (wave * WL + i) * 1024), 16, 0, 0);
+    for (int i = 0; i < WL; ++i) x8_copy(wr, d + (wave * WL + i) * 1024, wo[i], kb * kX8Block);
 #pragma unroll
-    for (int i = 0; i < XL; ++i)
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(xp[i] + kb * kX8Block),
-                                       (__attribute__((address_space(3))) void*)(d + BN * kX8Block + (wave * XL + i) * 1024),
-                                       16, 0, 0);
+    for (int i = 0; i < XL; ++i) x8_copy(xr, d + BN * kX8Block + (wave * XL + i) * 1024, xo[i], kb * kX8Block);
   };
   // this lane's rows of x: their scales
   const float* xsp[WT];
@@ -233,12 +279,20 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
   // the scale rows of the wave's features: one block of 128 (kX8Up: one of gate, one of up rows)
   const float *wsp0, *wsp1;
   if constexpr (MODE == kX8Up) {
-    wsp0 = ws + (int64_t)blockIdx.x * kblocks;
-    wsp1 = ws + (int64_t)(nblocks / 2 + blockIdx.x) * kblocks;
+    wsp0 = ws + (int64_t)tn * kblocks;
+    wsp1 = ws + (int64_t)(nblocks / 2 + tn) * kblocks;
   } else {
     static_assert(128 % (32 * WF) == 0, "a wave's features lie in one block");
     wsp0 = wsp1 = ws + (int64_t)min((n0 + wf * 32 * WF) / kX8Block, nblocks - 1) * kblocks;
   }
+  // scales of a step, loaded ahead of its copies: the wait for them is the barrier's
+  float xs[WT], sw0, sw1;
+  auto load_scales = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < WT; ++t) xs[t] = xsp[t][kb];
+    sw0 = wsp0[kb];
+    sw1 = wsp1[kb];
+  };
 
   f32x16 acc[WF][WT];
 #pragma unroll
@@ -248,25 +302,20 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[f][t][i] = 0.f;
 
-  auto operand = [&](const uint8_t* base, int r, int s) {  // 32 bytes of row r: chunks 4 s + 2 half, + 1
+  auto operand = [&](const uint8_t* base, int r, int s) __attribute__((always_inline)) {  // chunks 4 s + 2 half, + 1 of row r
     const int z = (r >> 1) & 7, c = 4 * s + 2 * half;
     const u32x4 lo = *reinterpret_cast<const u32x4*>(base + r * kX8Block + 16 * (c ^ z));
     const u32x4 hi = *reinterpret_cast<const u32x4*>(base + r * kX8Block + 16 * ((c + 1) ^ z));
     return join_x8(lo, hi);
   };
+  const bool live = wt * 32 * WT < rows;  // a wave whose rows are all past the last only copies
 
-  // scales of a step, loaded ahead of its copies: the wait for them is the barrier's
-  float xs[WT], sw0, sw1;
-  auto load_scales = [&](int kb) {
-#pragma unroll
-    for (int t = 0; t < WT; ++t) xs[t] = xsp[t][kb];
-    sw0 = wsp0[kb];
-    sw1 = wsp1[kb];
-  };
   load_scales(0);
-  issue(0, 0);
+  issue(0);
   for (int kb = 0; kb < kblocks; ++kb) {
-    __syncthreads();  // step kb is in LDS, step kb - 1 is done with
+    // step kb's copies are in LDS (a barrier alone does not wait for them), step kb - 1 is done with
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
     float s0[WT], s1[WT];
 #pragma unroll
     for (int t = 0; t < WT; ++t) {
@@ -275,9 +324,10 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
     }
     if (kb + 1 < kblocks) {
       load_scales(kb + 1);
-      issue(kb + 1, (kb + 1) & 1);
+      issue(kb + 1);
     }
-    const uint8_t* d = lds + (kb & 1) * kHalf;
+    if (!live) continue;
+    const uint8_t* d = lds + (kb & 1) * kStep;
     i32x8 b[WT][2];
 #pragma unroll
     for (int t = 0; t < WT; ++t)
@@ -299,12 +349,14 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
       }
     }
   }
+  __syncthreads();
 
   if constexpr (MODE == kX8Up) {
     // a = SiLU(gate) up, then one scale over the 128 features of a row: the
     // waves' parts of its largest value meet in LDS
-    __syncthreads();
-    float* top = reinterpret_cast<float*>(lds);  // [NF][BM]
+    float* top = reinterpret_cast<float*>(lds);               // [NF][BM]
+    uint8_t* stage = lds + NF * BM * 4;                       // [BM][128] quantised, chunks swizzled
+    static_assert(NF * BM * 4 + BM * 128 <= 2 * kStep, "both fit");
     constexpr int HF = WF / 2;
 #pragma unroll
     for (int t = 0; t < WT; ++t) {
@@ -331,9 +383,7 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
       for (int j = 0; j < NF; ++j) m = fmaxf(m, top[j * BM + r]);
       const uint32_t e = x8_scale_exp(m);
       const float inv = x8_inverse(e);
-      if (r >= rows) continue;
-      const int64_t p = first + r;
-      if (wf == 0 && half == 0) a.hs[p * (inter / kX8Block) + blockIdx.x] = x8_scale(e);
+      if (wf == 0 && half == 0 && r < rows) a.hs[(int64_t)(first + r) * (inter / kX8Block) + tn] = x8_scale(e);
 #pragma unroll
       for (int f = 0; f < HF; ++f)
 #pragma unroll
@@ -341,32 +391,52 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
           float v[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) v[i] = x8_value(acc[f][t][4 * q + i], inv);
-          *reinterpret_cast<uint32_t*>(a.h8 + p * inter + blockIdx.x * 128 + (wf * HF + f) * 32 + 8 * q + 4 * half) =
+          const int o = (wf * HF + f) * 32 + 8 * q + 4 * half;  // byte of the row
+          *reinterpret_cast<uint32_t*>(stage + r * 128 + (((o >> 4) ^ (r & 7)) << 4) + (o & 15)) =
               pack_x8(v[0], v[1], v[2], v[3]);
         }
     }
+    __syncthreads();
+    for (int u = tid; u < BM * 8; u += 64 * NW) {
+      const int r = u >> 3, c = u & 7;
+      if (r < rows)
+        *reinterpret_cast<u32x4*>(a.h8 + (int64_t)(first + r) * inter + tn * 128 + 16 * c) =
+            *reinterpret_cast<const u32x4*>(stage + r * 128 + 16 * (c ^ (r & 7)));
+    }
   } else {
+    // 32 rows x 64 features at a time through the wave's own LDS, out in whole rows' pieces
+    if (!live) return;
+    float* st = reinterpret_cast<float*>(lds + wave * kStage);
 #pragma unroll
     for (int t = 0; t < WT; ++t) {
-      const int r = (wt * WT + t) * 32 + l32;
-      if (r >= rows) continue;
-      int64_t row = first + r;
       float pw = 1.f;
       if constexpr (MODE == kX8Down) {
-        row = a.order[first + r];
-        pw = a.pair_w[row / a.top_k * a.pair_w_stride + row % a.top_k];
+        const int64_t pair = a.order[first + min((wt * WT + t) * 32 + l32, rows - 1)];
+        pw = a.pair_w[pair / a.top_k * a.pair_w_stride + pair % a.top_k];
       }
 #pragma unroll
-      for (int f = 0; f < WF; ++f)
+      for (int f0 = 0; f0 < WF; f0 += 2) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = n0 + (wf * WF + f) * 32 + 8 * q + 4 * half;
-          if (n >= a.n) continue;  // n is a multiple of 16: four features are in or out
-          float v[4];
+        for (int f = 0; f < 2; ++f)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = MODE == kX8Down ? pw * acc[f][t][4 * q + i] : acc[f][t][4 * q + i];
-          store_quad(a, row * a.y_stride + n, v);
+          for (int q = 0; q < 4; ++q) {
+            f32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = MODE == kX8Down ? pw * acc[f0 + f][t][4 * q + i] : acc[f0 + f][t][4 * q + i];
+            *reinterpret_cast<f32x4*>(st + l32 * kPitch + f * 32 + 8 * q + 4 * half) = v;
+          }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 8 * j + (lane >> 3), c = 8 * (lane & 7);
+          const f32x4 v0 = *reinterpret_cast<const f32x4*>(st + r * kPitch + c);
+          const f32x4 v1 = *reinterpret_cast<const f32x4*>(st + r * kPitch + c + 4);
+          const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+          const int rr = (wt * WT + t) * 32 + r, n = n0 + (wf * WF + f0) * 32 + c;
+          if (rr >= rows || n >= a.n) continue;  // n is a multiple of 16: eight features are in or out
+          const int64_t row = MODE == kX8Down ? a.order[first + rr] : first + rr;
+          store_eight(a, row * a.y_stride + n, v);
         }
+      }
     }
   }
 }
