@@ -13,44 +13,12 @@
 
 namespace ria {
 
-// One thread per 8 values, 16 threads per block of 128.
 template <int XT>
-__global__ __launch_bounds__(256) void quant_fp8_kernel(int64_t units, int per_row, const void* x, int64_t x_stride,
-                                                        uint8_t* out, float* scale) {
-  const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (u >= units) return;  // whole groups of 16 threads
-  const int64_t r = u / per_row;
-  const int c = static_cast<int>(u - r * per_row) * 8;
-  float v[8];
-  load_act8<XT>(x, r * x_stride + c, v);
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(v[i]));
-  const uint32_t e = x8_scale_exp(row16_max(top));
-  const float inv = x8_inverse(e);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = x8_value(v[i], inv);
-  *reinterpret_cast<u32x2*>(out + u * 8) = u32x2{pack_x8(v[0], v[1], v[2], v[3]), pack_x8(v[4], v[5], v[6], v[7])};
-  if ((threadIdx.x & 15) == 0) scale[u / 16] = x8_scale(e);
+__global__ __launch_bounds__(256) void quant_fp8_kernel(const QuantArgs a) {
+  quant_unit<XT>(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
 }
 
 bool x8_dtype_ok(int dt) { return dt == RIA_DT_BF16 || dt == RIA_DT_F16 || dt == RIA_DT_F32; }
-
-int launch_quant_fp8(const char* who, int64_t rows, int cols, const void* x, int x_dtype, int64_t x_row_stride,
-                     void* out, float* scale, hipStream_t st) {
-  const int64_t units = rows * (cols / 8), blocks = (units + 255) / 256;
-  if (blocks > 0x7fffffff) return set_error(RIA_ERR_INVALID, "%s: too many values", who);
-  const dim3 grid(static_cast<unsigned>(blocks));
-  uint8_t* o = static_cast<uint8_t*>(out);
-  if (x_dtype == RIA_DT_BF16)
-    hipLaunchKernelGGL((quant_fp8_kernel<RIA_DT_BF16>), grid, dim3(256), 0, st, units, cols / 8, x, x_row_stride, o, scale);
-  else if (x_dtype == RIA_DT_F16)
-    hipLaunchKernelGGL((quant_fp8_kernel<RIA_DT_F16>), grid, dim3(256), 0, st, units, cols / 8, x, x_row_stride, o, scale);
-  else
-    hipLaunchKernelGGL((quant_fp8_kernel<RIA_DT_F32>), grid, dim3(256), 0, st, units, cols / 8, x, x_row_stride, o, scale);
-  return check_launch(who);
-}
-
 
 }  // namespace ria
 
@@ -67,7 +35,18 @@ extern "C" int ria_quant_fp8(int64_t rows, int cols, const void* x, int x_dtype,
   if (x_row_stride < cols || x_row_stride % 8 || reinterpret_cast<uintptr_t>(x) % 16)
     return set_error(RIA_ERR_INVALID, "%s: x must be 16-byte aligned with a row stride of at least cols, a multiple of 8", who);
   if (reinterpret_cast<uintptr_t>(out) % 16) return set_error(RIA_ERR_INVALID, "%s: out must be 16-byte aligned", who);
-  return launch_quant_fp8(who, rows, cols, x, x_dtype, x_row_stride, out, scale, static_cast<hipStream_t>(stream));
+  const QuantArgs a{rows * (cols / 8), cols / 8, x, x_row_stride, static_cast<uint8_t*>(out), scale};
+  const int64_t blocks = (a.units + 255) / 256;
+  if (blocks > 0x7fffffff) return set_error(RIA_ERR_INVALID, "%s: too many values", who);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (x_dtype == RIA_DT_BF16)
+    hipLaunchKernelGGL((quant_fp8_kernel<RIA_DT_BF16>), grid, dim3(256), 0, st, a);
+  else if (x_dtype == RIA_DT_F16)
+    hipLaunchKernelGGL((quant_fp8_kernel<RIA_DT_F16>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((quant_fp8_kernel<RIA_DT_F32>), grid, dim3(256), 0, st, a);
+  return check_launch(who);
 }
 
 extern "C" int ria_linear_fp8_x8(int m, int n, int k, const void* x, int64_t x_row_stride, const float* x_scale,

@@ -205,51 +205,130 @@ static void launch_route(const RouteArgs& a, hipStream_t st) {
 
 // ----------------------------------------------------------------------------- experts
 constexpr int kMoeMaxExperts = 1024;
-constexpr int kMoeTile = 64;  // pairs of one expert in a tile
+constexpr int kPlanPairs = 4096;  // pairs a planning workgroup takes
+constexpr int kPlanPer = kPlanPairs / 256;
 
 struct PlanArgs {
   const int32_t* ids;
   int64_t id_stride;
-  int tokens, top_k, experts;
+  int pairs, top_k, experts;
+  int blocks;      // planning workgroups: ceil(pairs / kPlanPairs)
+  int tile;        // pairs of one expert in a tile
+  int32_t* counts; // [blocks, experts] (more than one workgroup)
   int32_t* order;
   X8Tile* tiles;
   int32_t* ntiles;
 };
 
-// One workgroup: a histogram of the experts, its running sums, and each pair's
-// place.  Ids outside [0, experts) are in no tile.
-__global__ __launch_bounds__(1024) void moe_plan_kernel(const PlanArgs a) {
-  __shared__ int count[kMoeMaxExperts], start[kMoeMaxExperts], tile0[kMoeMaxExperts];
+struct PlanShared {
+  int count[kMoeMaxExperts];  // pairs of the expert; then the next free position
+  int part[2][4];
+};
+
+// The experts of this thread's pairs (-1: none) and, in LDS, the workgroup's histogram.
+__device__ __forceinline__ void plan_count(const PlanArgs& a, int block, PlanShared& s, int (&e)[kPlanPer]) {
   const int tid = threadIdx.x;
-  const int pairs = a.tokens * a.top_k;
-  for (int e = tid; e < a.experts; e += 1024) count[e] = 0;
+  for (int i = tid; i < a.experts; i += 256) s.count[i] = 0;
   __syncthreads();
-  auto expert = [&](int p) { return a.ids[(int64_t)(p / a.top_k) * a.id_stride + p % a.top_k]; };
-  for (int p = tid; p < pairs; p += 1024) {
-    const int e = expert(p);
-    if (e >= 0 && e < a.experts) atomicAdd(&count[e], 1);
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) {
+    const int p = block * kPlanPairs + i * 256 + tid;
+    e[i] = -1;
+    if (p < a.pairs) e[i] = a.ids[(int64_t)(p / a.top_k) * a.id_stride + p % a.top_k];
+    if (e[i] >= a.experts) e[i] = -1;
   }
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i)
+    if (e[i] >= 0) atomicAdd(&s.count[e[i]], 1);
   __syncthreads();
-  if (tid == 0) {
-    int s = 0, n = 0;
-    for (int e = 0; e < a.experts; ++e) {
-      start[e] = s;
-      tile0[e] = n;
-      s += count[e];
-      n += (count[e] + kMoeTile - 1) / kMoeTile;
+}
+
+// Running sums of the experts' pairs and tiles (thread t: experts 4 t .. 4 t +
+// 3), this workgroup's first position of each expert, and its pairs' places.
+// Which of an expert's positions a pair gets does not change its results.
+__device__ __forceinline__ void plan_place(const PlanArgs& a, int block, PlanShared& s, const int (&e)[kPlanPer]) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int total[4], before[4], sum = 0, tiles = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int x = 4 * tid + j;
+    total[j] = before[j] = 0;
+    if (x < a.experts) {
+      if (a.blocks == 1) {
+        total[j] = s.count[x];
+      } else {
+        for (int b = 0; b < a.blocks; ++b) {
+          const int c = a.counts[b * a.experts + x];
+          before[j] += b < block ? c : 0;
+          total[j] += c;
+        }
+      }
     }
-    *a.ntiles = n;
+    sum += total[j];
+    tiles += (total[j] + a.tile - 1) / a.tile;
+  }
+  int run = sum, trun = tiles;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int u = __shfl_up(run, d), v = __shfl_up(trun, d);
+    if (lane >= d) {
+      run += u;
+      trun += v;
+    }
+  }
+  if (lane == 63) {
+    s.part[0][wave] = run;
+    s.part[1][wave] = trun;
   }
   __syncthreads();
-  for (int e = tid; e < a.experts; e += 1024) {
-    for (int i = 0; i * kMoeTile < count[e]; ++i)
-      a.tiles[tile0[e] + i] = X8Tile{e, start[e] + i * kMoeTile, min(kMoeTile, count[e] - i * kMoeTile), 0};
+  run -= sum;
+  trun -= tiles;
+  for (int w = 0; w < wave; ++w) {
+    run += s.part[0][w];
+    trun += s.part[1][w];
+  }
+  if (block == 0 && tid == 255) *a.ntiles = trun + tiles;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int x = 4 * tid + j;
+    if (x < a.experts) {
+      s.count[x] = run + before[j];
+      if (block == 0)
+        for (int i = 0; i < total[j]; i += a.tile)
+          a.tiles[trun++] = X8Tile{x, run + i, min(a.tile, total[j] - i), 0};
+      run += total[j];
+    }
   }
   __syncthreads();
-  for (int p = tid; p < pairs; p += 1024) {
-    const int e = expert(p);
-    if (e >= 0 && e < a.experts) a.order[atomicAdd(&start[e], 1)] = p;
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i)
+    if (e[i] >= 0) a.order[atomicAdd(&s.count[e[i]], 1)] = block * kPlanPairs + i * 256 + tid;
+}
+
+// First launch: workgroups 0 .. blocks - 1 count their pairs' experts (a lone
+// one places them too), the others quantise x.
+template <int XT>
+__global__ __launch_bounds__(256) void moe_prepare_kernel(const PlanArgs a, const QuantArgs q) {
+  __shared__ PlanShared s;
+  if (static_cast<int>(blockIdx.x) >= a.blocks) {
+    quant_unit<XT>(q, (int64_t)(blockIdx.x - a.blocks) * 256 + threadIdx.x);
+    return;
   }
+  const int block = blockIdx.x;
+  int e[kPlanPer];
+  plan_count(a, block, s, e);
+  if (a.blocks == 1) {
+    plan_place(a, 0, s, e);
+  } else {
+    for (int i = threadIdx.x; i < a.experts; i += 256) a.counts[block * a.experts + i] = s.count[i];
+  }
+}
+
+__global__ __launch_bounds__(256) void moe_place_kernel(const PlanArgs a) {
+  __shared__ PlanShared s;
+  int e[kPlanPer];
+  plan_count(a, blockIdx.x, s, e);
+  plan_place(a, blockIdx.x, s, e);
 }
 
 struct CombineArgs {
@@ -293,12 +372,17 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs a) {
 static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // Most tiles of any routing: an expert's last tile may be partly filled.
-static int64_t moe_tiles(int64_t pairs, int experts) {
-  return std::min<int64_t>(pairs, pairs / kMoeTile + std::min<int64_t>(experts, pairs));
+static int64_t moe_tiles(int64_t pairs, int experts, int tile) {
+  return std::min<int64_t>(pairs, pairs / tile + std::min<int64_t>(experts, pairs));
+}
+
+// Pairs of one expert that a tile takes.
+static int moe_tile(int64_t pairs, int experts, int out_dtype) {
+  return out_dtype != RIA_DT_F32 && pairs >= (int64_t)experts * 128 ? 256 : 64;
 }
 
 struct MoeLayout {
-  int64_t x8, xs, order, tiles, ntiles, h8, hs, slots, bytes;
+  int64_t x8, xs, counts, order, tiles, ntiles, h8, hs, slots, bytes;
 };
 static MoeLayout moe_layout(int64_t tokens, int top_k, int experts, int hidden, int inter, int out_dtype) {
   MoeLayout l{};
@@ -311,8 +395,9 @@ static MoeLayout moe_layout(int64_t tokens, int top_k, int experts, int hidden, 
   };
   l.x8 = take(tokens * hidden);
   l.xs = take(tokens * (hidden / kX8Block) * 4);
+  l.counts = take((pairs + kPlanPairs - 1) / kPlanPairs * experts * 4);
   l.order = take(pairs * 4);
-  l.tiles = take(moe_tiles(pairs, experts) * static_cast<int64_t>(sizeof(X8Tile)));
+  l.tiles = take(moe_tiles(pairs, experts, moe_tile(pairs, experts, out_dtype)) * static_cast<int64_t>(sizeof(X8Tile)));
   l.ntiles = take(4);
   l.h8 = take(pairs * inter);
   l.hs = take(pairs * (inter / kX8Block) * 4);
@@ -402,14 +487,24 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
   int32_t* order = static_cast<int32_t*>(at(l.order));
   X8Tile* tiles = static_cast<X8Tile*>(at(l.tiles));
   int32_t* ntiles = static_cast<int32_t*>(at(l.ntiles));
-  const int64_t pairs = (int64_t)d->tokens * d->top_k, most = moe_tiles(pairs, d->experts);
+  const int64_t pairs = (int64_t)d->tokens * d->top_k;
+  const int tile = moe_tile(pairs, d->experts, d->out_dtype);
+  const int64_t most = moe_tiles(pairs, d->experts, tile);
   if (most * (std::max(d->hidden, d->inter) / 128) > 0x7ffffff0)
     return set_error(RIA_ERR_INVALID, "%s: too many (token, slot) pairs", who);
-  if (int rc = launch_quant_fp8(who, d->tokens, d->hidden, d->x, d->x_dtype, d->x_row_stride, at(l.x8),
-                                static_cast<float*>(at(l.xs)), st))
-    return rc;
-  const PlanArgs plan{d->ids, d->ids_row_stride, d->tokens, d->top_k, d->experts, order, tiles, ntiles};
-  hipLaunchKernelGGL(moe_plan_kernel, dim3(1), dim3(1024), 0, st, plan);
+  const PlanArgs plan{d->ids, d->ids_row_stride, static_cast<int>(pairs), d->top_k, d->experts,
+                      static_cast<int>((pairs + kPlanPairs - 1) / kPlanPairs), tile, static_cast<int32_t*>(at(l.counts)),
+                      order, tiles, ntiles};
+  const QuantArgs quant{d->tokens * (int64_t)(d->hidden / 8), d->hidden / 8, d->x, d->x_row_stride,
+                        static_cast<uint8_t*>(at(l.x8)), static_cast<float*>(at(l.xs))};
+  const dim3 pgrid(static_cast<unsigned>(plan.blocks + (quant.units + 255) / 256));
+  if (d->x_dtype == RIA_DT_BF16)
+    hipLaunchKernelGGL((moe_prepare_kernel<RIA_DT_BF16>), pgrid, dim3(256), 0, st, plan, quant);
+  else if (d->x_dtype == RIA_DT_F16)
+    hipLaunchKernelGGL((moe_prepare_kernel<RIA_DT_F16>), pgrid, dim3(256), 0, st, plan, quant);
+  else
+    hipLaunchKernelGGL((moe_prepare_kernel<RIA_DT_F32>), pgrid, dim3(256), 0, st, plan, quant);
+  if (plan.blocks > 1) hipLaunchKernelGGL(moe_place_kernel, dim3(plan.blocks), dim3(256), 0, st, plan);
   X8Args up{};
   up.x = static_cast<const uint8_t*>(at(l.x8));
   up.x_stride = d->hidden;
@@ -430,6 +525,8 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
   auto grid_of = [&](int feature_tiles) { return dim3(static_cast<unsigned>((most * feature_tiles + 7) / 8 * 8)); };
   if (wide)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true>), grid_of(d->inter / 128), dim3(256), 0, st, up);
+  else if (tile == 256)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 4, 2, 2, 4, false>), grid_of(d->inter / 128), dim3(512), 0, st, up);
   else
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false>), grid_of(d->inter / 128), dim3(256), 0, st, up);
   X8Args dn = up;
@@ -449,6 +546,8 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
   dn.pair_w_stride = d->weights_row_stride;
   if (wide)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, true>), grid_of(d->hidden / 128), dim3(256), 0, st, dn);
+  else if (tile == 256)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 4, 2, 2, 4, false>), grid_of((d->hidden + 255) / 256), dim3(512), 0, st, dn);
   else
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, false>), grid_of(d->hidden / 128), dim3(256), 0, st, dn);
   const CombineArgs c{at(l.slots), d->ids, d->ids_row_stride, d->tokens, d->top_k, d->experts, d->hidden, d->out,

@@ -96,6 +96,34 @@ __device__ __forceinline__ float row16_max(float v) {
   return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true)));
 }
 
+struct QuantArgs {
+  int64_t units;     // rows * per_row
+  int per_row;       // 8 values each
+  const void* x;
+  int64_t x_stride;
+  uint8_t* out;
+  float* scale;
+};
+
+// One thread per 8 values, 16 threads per block of 128 (units are whole blocks).
+template <int XT>
+__device__ __forceinline__ void quant_unit(const QuantArgs& a, int64_t u) {
+  if (u >= a.units) return;
+  const int64_t r = u / a.per_row;
+  const int c = static_cast<int>(u - r * a.per_row) * 8;
+  float v[8];
+  load_act8<XT>(a.x, r * a.x_stride + c, v);
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(v[i]));
+  const uint32_t e = x8_scale_exp(row16_max(top));
+  const float inv = x8_inverse(e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = x8_value(v[i], inv);
+  *reinterpret_cast<u32x2*>(a.out + u * 8) = u32x2{pack_x8(v[0], v[1], v[2], v[3]), pack_x8(v[4], v[5], v[6], v[7])};
+  if ((u & 15) == 0) a.scale[u / 16] = x8_scale(e);
+}
+
 // ---- the tiled product
 enum X8Mode {
   kX8Dense = 0,  // y [m, n]
@@ -443,7 +471,5 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
 
 // Host side (linear_x8.hip).
 bool x8_dtype_ok(int dt);
-int launch_quant_fp8(const char* who, int64_t rows, int cols, const void* x, int x_dtype, int64_t x_row_stride,
-                     void* out, float* scale, hipStream_t st);
 
 }  // namespace ria
