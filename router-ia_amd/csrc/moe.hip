@@ -331,6 +331,312 @@ __global__ __launch_bounds__(256) void moe_place_kernel(const PlanArgs a) {
   plan_place(a, blockIdx.x, s, e);
 }
 
+// ---- few tokens: the weights stream through registers
+//
+// A decode batch leaves an expert a handful of tokens, so the time is the
+// weights' way from HBM: each is read once, straight into MFMA operands (16
+// rows x 128 bytes of K per product, widened to fp16), by many small
+// workgroups with all of their loads in flight.  A tile is up to 16 tokens of
+// one expert, the 16 columns of a product.
+constexpr int kFewTile = 16;
+constexpr int kFewAhead = 4;      // blocks of K a wave loads at once
+constexpr int kFewChunk = 2048;   // hidden values quantised into LDS at a time
+
+struct FewArgs {
+  const int32_t* order;           // tiles of the plan, or (pairs mode) each pair its own tile
+  const X8Tile* tiles;
+  const int32_t* ntiles;
+  const int32_t* ids;
+  int64_t id_stride;
+  const void* x;                  // pairs mode: x itself
+  int64_t x_stride;
+  const uint8_t* x8;
+  const float* xs;
+  const float* pair_w;
+  int64_t pair_w_stride;
+  int tokens, top_k, experts, hidden, inter;
+  const uint8_t* w13;
+  const float* s13;
+  const uint8_t* w2;
+  const float* s2;
+  float* act;                     // [positions or pairs, inter]: SiLU(g) u
+  void* slots;
+  int slot_dtype;
+  void* out;                      // pairs mode: the sums
+  int64_t out_stride;
+  int out_dtype, add;
+};
+
+// 16 rows of w at block kb of K: this lane's 32 bytes (row l % 16, part l / 16).
+__device__ __forceinline__ void load_rows16(const uint8_t* w, int k, int kb, int lane, u32x4 (&v)[2]) {
+  const u32x4* p = reinterpret_cast<const u32x4*>(w + (int64_t)(lane & 15) * k + kb * kX8Block + 32 * (lane >> 4));
+  v[0] = ld_stream(p);
+  v[1] = ld_stream(p + 1);
+}
+
+// act = SiLU(g) u of one tile and 16 features, four waves sharing K.  PAIRS:
+// the tile is one (token, slot) pair, and x is quantised here.
+template <int XT, bool PAIRS>
+__global__ __launch_bounds__(256) void moe_up_few_kernel(const FewArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t xq_s[];  // PAIRS: hidden e4m3 values, then their scales
+  __shared__ f32x4 red[4][2][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int groups = a.inter / 16;
+  const int tile = blockIdx.x / groups, c0 = blockIdx.x % groups * 16;
+  int expert, first, rows = 1;
+  if constexpr (PAIRS) {
+    first = tile;
+    expert = a.ids[(int64_t)(tile / a.top_k) * a.id_stride + tile % a.top_k];
+    if (expert < 0 || expert >= a.experts) return;
+  } else {
+    if (tile >= *a.ntiles) return;
+    const X8Tile t = a.tiles[tile];
+    expert = t.expert;
+    first = t.first;
+    rows = t.rows;
+  }
+  expert = __builtin_amdgcn_readfirstlane(expert);
+  const int k = a.hidden, kblocks = k / kX8Block;
+  const uint8_t* wg = a.w13 + ((int64_t)expert * 2 * a.inter + c0) * k;
+  const uint8_t* wu = wg + (int64_t)a.inter * k;
+  const float* sg = a.s13 + ((int64_t)expert * 2 * (a.inter / kX8Block) + c0 / kX8Block) * kblocks;
+  const float* su = sg + (int64_t)(a.inter / kX8Block) * kblocks;
+  const int at = first + min(lane & 15, rows - 1);
+  const int64_t token = PAIRS ? tile / a.top_k : a.order[at] / a.top_k;
+  const uint8_t* x8 = a.x8 + token * k + 32 * (lane >> 4);
+  const float* xs = a.xs + token * kblocks;
+
+  u32x4 g[kFewAhead][2], u[kFewAhead][2];
+  auto load = [&](int kb0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int kb = min(kb0 + i, kblocks - 1);
+      load_rows16(wg, k, kb, lane, g[i]);
+      load_rows16(wu, k, kb, lane, u[i]);
+    }
+  };
+  load(wave * kFewAhead);
+  if constexpr (PAIRS) {
+    uint8_t* q = xq_s;
+    float* qs = reinterpret_cast<float*>(xq_s + k);
+    const int64_t x0 = token * a.x_stride;
+    for (int c = 8 * tid; c < k; c += 8 * 256) {
+      float v[8];
+      load_act8<XT>(a.x, x0 + c, v);
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(v[i]));
+      const uint32_t e = x8_scale_exp(row16_max(top));
+      const float inv = x8_inverse(e);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = x8_value(v[i], inv);
+      *reinterpret_cast<u32x2*>(q + c) = u32x2{pack_x8(v[0], v[1], v[2], v[3]), pack_x8(v[4], v[5], v[6], v[7])};
+      if ((c & (kX8Block - 1)) == 0) qs[c / kX8Block] = x8_scale(e);
+    }
+    lds_barrier();
+  }
+  f32x4 ag{0.f, 0.f, 0.f, 0.f}, au = ag;
+  for (int kb0 = wave * kFewAhead; kb0 < kblocks; kb0 += 4 * kFewAhead) {
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int kb = kb0 + i;
+      if (kb >= kblocks) break;
+      u32x4 b[2];
+      float s;
+      if constexpr (PAIRS) {
+        const u32x4* p = reinterpret_cast<const u32x4*>(xq_s + kb * kX8Block + 32 * (lane >> 4));
+        b[0] = p[0];
+        b[1] = p[1];
+        s = reinterpret_cast<const float*>(xq_s + k)[kb];
+      } else {
+        const u32x4* p = reinterpret_cast<const u32x4*>(x8 + kb * kX8Block);
+        b[0] = p[0];
+        b[1] = p[1];
+        s = xs[kb];
+      }
+      const f32x4 pg = mfma_x8_16(g[i], b), pu = mfma_x8_16(u[i], b);
+      const float fg = s * sg[kb], fu = s * su[kb];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ag[j] = fmaf(pg[j], fg, ag[j]);
+        au[j] = fmaf(pu[j], fu, au[j]);
+      }
+    }
+    if (kb0 + 4 * kFewAhead < kblocks) load(kb0 + 4 * kFewAhead);
+  }
+  red[wave][0][lane] = ag;
+  red[wave][1][lane] = au;
+  __syncthreads();
+  // thread (row, feature): result (feature, row) of the products is value feature % 4 of lane row + 16 (feature / 4)
+  const int row = tid >> 4, f = tid & 15;
+  if (row >= rows) return;
+  float gate = 0.f, up = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    gate += red[w][0][row + 16 * (f >> 2)][f & 3];
+    up += red[w][1][row + 16 * (f >> 2)][f & 3];
+  }
+  a.act[(int64_t)(first + row) * a.inter + c0 + f] = x8_swiglu(gate, up);
+}
+
+// 8 values of act to e4m3 at d, their block's scale to s (16 lanes a block).
+__device__ __forceinline__ void quant_act8(const float* p, uint8_t* d, float* s, int lane) {
+  const f32x4 v0 = *reinterpret_cast<const f32x4*>(p), v1 = *reinterpret_cast<const f32x4*>(p + 4);
+  float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(v[i]));
+  const uint32_t e = x8_scale_exp(row16_max(top));
+  const float inv = x8_inverse(e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = x8_value(v[i], inv);
+  *reinterpret_cast<u32x2*>(d) = u32x2{pack_x8(v[0], v[1], v[2], v[3]), pack_x8(v[4], v[5], v[6], v[7])};
+  if ((lane & 15) == 0) *s = x8_scale(e);
+}
+
+// One tile's rows of 128 features of the output (a wave: 32 of them), to the
+// pairs' slots.
+__global__ __launch_bounds__(256) void moe_down_few_kernel(const FewArgs a) {
+  constexpr int kPitch = kFewChunk + 16;  // 16 rows' reads meet all banks
+  __shared__ __attribute__((aligned(16))) uint8_t h_s[kFewTile * kPitch];
+  __shared__ float hs_s[kFewTile][kFewChunk / kX8Block];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int groups = a.hidden / 128;
+  const int tile = blockIdx.x / groups;
+  if (tile >= *a.ntiles) return;
+  const X8Tile t = a.tiles[tile];
+  const int expert = __builtin_amdgcn_readfirstlane(t.expert), rows = __builtin_amdgcn_readfirstlane(t.rows);
+  const int n0 = blockIdx.x % groups * 128 + wave * 32;
+  const int k = a.inter, kblocks = k / kX8Block;
+  const uint8_t* w = a.w2 + ((int64_t)expert * a.hidden + n0) * k;
+  const float* s2 = a.s2 + ((int64_t)expert * groups + blockIdx.x % groups) * kblocks;
+  u32x4 v[2][kFewAhead][2];
+  auto load = [&](int kb0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int kb = min(kb0 + i, kblocks - 1);
+      load_rows16(w, k, kb, lane, v[0][i]);
+      load_rows16(w + (int64_t)16 * k, k, kb, lane, v[1][i]);
+    }
+  };
+  load(0);
+  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  for (int c0 = 0; c0 < k; c0 += kFewChunk) {
+    const int cols = min(kFewChunk, k - c0), units = cols / 8;
+    if (c0) __syncthreads();
+    for (int u = tid; u < rows * units; u += 256) {
+      const int r = u / units, c = (u - r * units) * 8;
+      quant_act8(a.act + (int64_t)(t.first + r) * k + c0 + c, h_s + r * kPitch + c, &hs_s[r][c / kX8Block], tid);
+    }
+    lds_barrier();
+    const int row = min(lane & 15, rows - 1);
+    for (int b0 = 0; b0 < cols / kX8Block; b0 += kFewAhead) {
+#pragma unroll
+      for (int i = 0; i < kFewAhead; ++i) {
+        const int kb = b0 + i;  // of the chunk
+        if (kb >= cols / kX8Block) break;
+        const u32x4* p = reinterpret_cast<const u32x4*>(h_s + row * kPitch + kb * kX8Block + 32 * (lane >> 4));
+        const u32x4 b[2] = {p[0], p[1]};
+        const float s = hs_s[row][kb] * s2[c0 / kX8Block + kb];
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          const f32x4 part = mfma_x8_16(v[f][i], b);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[f][j] = fmaf(part[j], s, acc[f][j]);
+        }
+      }
+      const int next = c0 / kX8Block + b0 + kFewAhead;
+      if (next < kblocks) load(next);
+    }
+  }
+  if ((lane & 15) >= rows) return;
+  const int64_t pair = a.order[t.first + (lane & 15)];
+  const float pw = a.pair_w[pair / a.top_k * a.pair_w_stride + pair % a.top_k];
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+    const int64_t o = pair * a.hidden + n0 + 16 * f + 4 * (lane >> 4);
+    float r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = pw * acc[f][j];
+    if (a.slot_dtype == RIA_DT_F32)
+      store_act4<RIA_DT_F32>(a.slots, o, r);
+    else if (a.slot_dtype == RIA_DT_F16)
+      store_act4<RIA_DT_F16>(a.slots, o, r);
+    else
+      store_act4<RIA_DT_BF16>(a.slots, o, r);
+  }
+}
+
+// Pairs mode: 16 features of one token's sum, a wave for each slot (in turns of
+// kSumWaves); the terms meet in LDS and are added in slot order.
+constexpr int kSumWaves = 8;
+template <int DT>
+__global__ __launch_bounds__(64 * kSumWaves) void moe_down_pairs_kernel(const FewArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t h_s[kSumWaves][kFewChunk];
+  __shared__ float hs_s[kSumWaves][kFewChunk / kX8Block];
+  __shared__ float term[kSumWaves][16];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int groups = a.hidden / 16;
+  const int t = blockIdx.x / groups, n0 = blockIdx.x % groups * 16;
+  const int k = a.inter, kblocks = k / kX8Block;
+  float sum = 0.f;  // thread f < 16: feature n0 + f
+  for (int j0 = 0; j0 < a.top_k; j0 += kSumWaves) {
+    const int j = j0 + wave;
+    int expert = j < a.top_k ? a.ids[(int64_t)t * a.id_stride + j] : -1;
+    expert = __builtin_amdgcn_readfirstlane(expert);
+    const bool some = expert >= 0 && expert < a.experts;
+    f32x4 acc{0.f, 0.f, 0.f, 0.f};
+    if (some) {
+      const uint8_t* w = a.w2 + ((int64_t)expert * a.hidden + n0) * k;
+      const float* s2 = a.s2 + ((int64_t)expert * (a.hidden / kX8Block) + n0 / kX8Block) * kblocks;
+      const float* act = a.act + ((int64_t)t * a.top_k + j) * k;
+      for (int c0 = 0; c0 < k; c0 += kFewChunk) {
+        const int cols = min(kFewChunk, k - c0);
+        for (int b0 = 0; b0 < cols / kX8Block; b0 += kFewAhead) {
+          u32x4 v[kFewAhead][2];
+#pragma unroll
+          for (int i = 0; i < kFewAhead; ++i) load_rows16(w, k, min(c0 / kX8Block + b0 + i, kblocks - 1), lane, v[i]);
+          if (b0 == 0)  // 64 lanes: four blocks at a time (whole groups of 16 lanes)
+            for (int c = 8 * lane; c < cols; c += 8 * 64)
+              quant_act8(act + c0 + c, h_s[wave] + c, &hs_s[wave][c / kX8Block], lane);
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int i = 0; i < kFewAhead; ++i) {
+            const int kb = b0 + i;
+            if (kb >= cols / kX8Block) break;
+            const u32x4* p = reinterpret_cast<const u32x4*>(h_s[wave] + kb * kX8Block + 32 * (lane >> 4));
+            const u32x4 b[2] = {p[0], p[1]};
+            const float s = hs_s[wave][kb] * s2[c0 / kX8Block + kb];
+            const f32x4 part = mfma_x8_16(v[i], b);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[q] = fmaf(part[q], s, acc[q]);
+          }
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+    }
+    if ((lane & 15) == 0) {  // column 0: every column is the pair's
+      const float pw = some ? a.pair_w[(int64_t)t * a.pair_w_stride + j] : 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) term[wave][4 * (lane >> 4) + q] = some ? through_dtype<DT>(pw * acc[q]) : 0.f;
+    }
+    __syncthreads();
+    if (tid < 16)
+      for (int w = 0; w < min(kSumWaves, a.top_k - j0); ++w) sum = add_rn(sum, term[w][tid]);
+    __syncthreads();
+  }
+  if (tid < 16) {
+    const int64_t o = (int64_t)t * a.out_stride + n0 + tid;
+    if constexpr (DT == RIA_DT_F32) {
+      if (a.add) sum = add_rn(static_cast<const float*>(a.out)[o], sum);
+    }
+    store_act<DT>(a.out, o, sum);
+  }
+}
+
 struct CombineArgs {
   const void* slots;  // [tokens * top_k, hidden], in out's dtype
   const int32_t* ids;
@@ -338,35 +644,42 @@ struct CombineArgs {
   int tokens, top_k, experts, hidden;
   void* out;
   int64_t out_stride;
-  int add;
+  int add, vec;
 };
+constexpr int kCombineAhead = 4;  // slots loaded ahead of their sums
 
 // out[t] (+)= the sum of the token's slots in slot order, in fp32; slots of no
 // expert were never written and are left out.
 template <int DT>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs a) {
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int per = a.hidden / 4;
+  const int per = a.hidden / 8;
   const int64_t t = u / per;
   if (t >= a.tokens) return;
-  const int c = static_cast<int>(u - t * per) * 4;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < a.top_k; ++j) {
-    const int e = a.ids[t * a.id_stride + j];
-    if (e < 0 || e >= a.experts) continue;
-    float v[4];
-    load_act4<DT>(a.slots, (t * a.top_k + j) * a.hidden + c, v);
+  const int c = static_cast<int>(u - t * per) * 8;
+  float s[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = add_rn(s[i], v[i]);
-  }
+  for (int i = 0; i < 8; ++i) s[i] = 0.f;
+  for (int j0 = 0; j0 < a.top_k; j0 += kCombineAhead) {
+    float v[kCombineAhead][8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t o = t * a.out_stride + c + i;
-    if constexpr (DT == RIA_DT_F32) {
-      if (a.add) s[i] = add_rn(static_cast<const float*>(a.out)[o], s[i]);
+    for (int j = 0; j < kCombineAhead; ++j) {
+      const int e = j0 + j < a.top_k ? a.ids[t * a.id_stride + j0 + j] : -1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] = 0.f;
+      if (e >= 0 && e < a.experts) load_act8<DT>(a.slots, (t * a.top_k + j0 + j) * a.hidden + c, v[j]);
     }
-    store_act<DT>(a.out, o, s[i]);
+#pragma unroll
+    for (int j = 0; j < kCombineAhead; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = add_rn(s[i], v[j][i]);
   }
+  X8Args o{};
+  o.y = a.out;
+  o.y_dtype = DT;
+  o.y_add = a.add;
+  o.vec = a.vec;
+  store_eight(o, t * a.out_stride + c, s);
 }
 
 static int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
@@ -376,13 +689,22 @@ static int64_t moe_tiles(int64_t pairs, int experts, int tile) {
   return std::min<int64_t>(pairs, pairs / tile + std::min<int64_t>(experts, pairs));
 }
 
+// How a call is run, by its pairs: each pair by itself, tiles of 16 pairs whose
+// weights stream through registers, or tiles of 64 or 256 pairs in LDS.
+enum class MoeKind { kPairs, kFew, kTiles };
+static MoeKind moe_kind(int64_t pairs, int experts) {
+  if (pairs <= 32) return MoeKind::kPairs;
+  return pairs <= (int64_t)experts * 8 ? MoeKind::kFew : MoeKind::kTiles;
+}
+
 // Pairs of one expert that a tile takes.
 static int moe_tile(int64_t pairs, int experts, int out_dtype) {
+  if (moe_kind(pairs, experts) != MoeKind::kTiles) return kFewTile;
   return out_dtype != RIA_DT_F32 && pairs >= (int64_t)experts * 128 ? 256 : 64;
 }
 
 struct MoeLayout {
-  int64_t x8, xs, counts, order, tiles, ntiles, h8, hs, slots, bytes;
+  int64_t x8, xs, counts, order, tiles, ntiles, act, h8, hs, slots, bytes;
 };
 static MoeLayout moe_layout(int64_t tokens, int top_k, int experts, int hidden, int inter, int out_dtype) {
   MoeLayout l{};
@@ -399,11 +721,64 @@ static MoeLayout moe_layout(int64_t tokens, int top_k, int experts, int hidden, 
   l.order = take(pairs * 4);
   l.tiles = take(moe_tiles(pairs, experts, moe_tile(pairs, experts, out_dtype)) * static_cast<int64_t>(sizeof(X8Tile)));
   l.ntiles = take(4);
-  l.h8 = take(pairs * inter);
-  l.hs = take(pairs * (inter / kX8Block) * 4);
+  const bool tiled = moe_kind(pairs, experts) == MoeKind::kTiles;
+  l.act = take(tiled ? 0 : pairs * inter * 4);
+  l.h8 = take(tiled ? pairs * inter : 0);
+  l.hs = take(tiled ? pairs * (inter / kX8Block) * 4 : 0);
   l.slots = take(pairs * hidden * (out_dtype == RIA_DT_F32 ? 4 : 2));
   l.bytes = at;
   return l;
+}
+
+// The tiled kernels: gate and up rows, then down rows, of `most` tiles at the most.
+static void launch_moe_tiles(const ria_moe_experts_desc& d, const MoeLayout& l, int64_t most, int tile, hipStream_t st) {
+  char* ws = static_cast<char*>(d.workspace);
+  auto at = [&](int64_t o) { return static_cast<void*>(ws + o); };
+  X8Args up{};
+  up.x = static_cast<const uint8_t*>(at(l.x8));
+  up.x_stride = d.hidden;
+  up.xs = static_cast<const float*>(at(l.xs));
+  up.xs_stride = d.hidden / kX8Block;
+  up.w = static_cast<const uint8_t*>(d.w13);
+  up.ws = d.w13_scale_inv;
+  up.n = 2 * d.inter;
+  up.k = d.hidden;
+  up.order = static_cast<const int32_t*>(at(l.order));
+  up.tiles = static_cast<const X8Tile*>(at(l.tiles));
+  up.ntiles = static_cast<const int32_t*>(at(l.ntiles));
+  up.top_k = d.top_k;
+  up.h8 = static_cast<uint8_t*>(at(l.h8));
+  up.hs = static_cast<float*>(at(l.hs));
+  up.m = d.tokens;
+  const bool wide = d.out_dtype == RIA_DT_F32;
+  auto grid_of = [&](int feature_tiles) { return dim3(static_cast<unsigned>((most * feature_tiles + 7) / 8 * 8)); };
+  if (wide)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
+  else if (tile == 256)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 4, 2, 2, 4, false>), grid_of(d.inter / 128), dim3(512), 0, st, up);
+  else
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false>), grid_of(d.inter / 128), dim3(256), 0, st, up);
+  X8Args dn = up;
+  dn.x = up.h8;
+  dn.x_stride = d.inter;
+  dn.xs = up.hs;
+  dn.xs_stride = d.inter / kX8Block;
+  dn.w = static_cast<const uint8_t*>(d.w2);
+  dn.ws = d.w2_scale_inv;
+  dn.n = d.hidden;
+  dn.k = d.inter;
+  dn.y = at(l.slots);
+  dn.y_stride = d.hidden;
+  dn.y_dtype = d.out_dtype;
+  dn.vec = 1;
+  dn.pair_w = d.weights;
+  dn.pair_w_stride = d.weights_row_stride;
+  if (wide)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, true>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
+  else if (tile == 256)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 4, 2, 2, 4, false>), grid_of((d.hidden + 255) / 256), dim3(512), 0, st, dn);
+  else
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, false>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
 }
 
 static const char* moe_sizes_error(int64_t tokens, int top_k, int experts, int hidden, int inter) {
@@ -488,10 +863,35 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
   X8Tile* tiles = static_cast<X8Tile*>(at(l.tiles));
   int32_t* ntiles = static_cast<int32_t*>(at(l.ntiles));
   const int64_t pairs = (int64_t)d->tokens * d->top_k;
+  const MoeKind kind = moe_kind(pairs, d->experts);
   const int tile = moe_tile(pairs, d->experts, d->out_dtype);
   const int64_t most = moe_tiles(pairs, d->experts, tile);
-  if (most * (std::max(d->hidden, d->inter) / 128) > 0x7ffffff0)
+  if (std::max(most, pairs) * (std::max(d->hidden, d->inter) / 16) > 0x7ffffff0)
     return set_error(RIA_ERR_INVALID, "%s: too many (token, slot) pairs", who);
+  FewArgs few{order, tiles, ntiles, d->ids, d->ids_row_stride, d->x, d->x_row_stride,
+              static_cast<const uint8_t*>(at(l.x8)), static_cast<const float*>(at(l.xs)), d->weights,
+              d->weights_row_stride, d->tokens, d->top_k, d->experts, d->hidden, d->inter,
+              static_cast<const uint8_t*>(d->w13), d->w13_scale_inv, static_cast<const uint8_t*>(d->w2),
+              d->w2_scale_inv, static_cast<float*>(at(l.act)), at(l.slots), d->out_dtype, d->out, d->out_row_stride,
+              d->out_dtype, d->accumulate != 0};
+  if (kind == MoeKind::kPairs) {
+    const dim3 ugrid(static_cast<unsigned>(pairs * (d->inter / 16)));
+    const dim3 dgrid(static_cast<unsigned>((int64_t)d->tokens * (d->hidden / 16)));
+    const size_t lds = d->hidden + d->hidden / kX8Block * 4;
+    if (d->x_dtype == RIA_DT_BF16)
+      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_BF16, true>), ugrid, dim3(256), lds, st, few);
+    else if (d->x_dtype == RIA_DT_F16)
+      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F16, true>), ugrid, dim3(256), lds, st, few);
+    else
+      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F32, true>), ugrid, dim3(256), lds, st, few);
+    if (d->out_dtype == RIA_DT_BF16)
+      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_BF16>), dgrid, dim3(64 * kSumWaves), 0, st, few);
+    else if (d->out_dtype == RIA_DT_F16)
+      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_F16>), dgrid, dim3(64 * kSumWaves), 0, st, few);
+    else
+      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_F32>), dgrid, dim3(64 * kSumWaves), 0, st, few);
+    return check_launch(who);
+  }
   const PlanArgs plan{d->ids, d->ids_row_stride, static_cast<int>(pairs), d->top_k, d->experts,
                       static_cast<int>((pairs + kPlanPairs - 1) / kPlanPairs), tile, static_cast<int32_t*>(at(l.counts)),
                       order, tiles, ntiles};
@@ -505,54 +905,17 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
   else
     hipLaunchKernelGGL((moe_prepare_kernel<RIA_DT_F32>), pgrid, dim3(256), 0, st, plan, quant);
   if (plan.blocks > 1) hipLaunchKernelGGL(moe_place_kernel, dim3(plan.blocks), dim3(256), 0, st, plan);
-  X8Args up{};
-  up.x = static_cast<const uint8_t*>(at(l.x8));
-  up.x_stride = d->hidden;
-  up.xs = static_cast<const float*>(at(l.xs));
-  up.xs_stride = d->hidden / kX8Block;
-  up.w = static_cast<const uint8_t*>(d->w13);
-  up.ws = d->w13_scale_inv;
-  up.n = 2 * d->inter;
-  up.k = d->hidden;
-  up.order = order;
-  up.tiles = tiles;
-  up.ntiles = ntiles;
-  up.top_k = d->top_k;
-  up.h8 = static_cast<uint8_t*>(at(l.h8));
-  up.hs = static_cast<float*>(at(l.hs));
-  up.m = d->tokens;
-  const bool wide = d->out_dtype == RIA_DT_F32;
-  auto grid_of = [&](int feature_tiles) { return dim3(static_cast<unsigned>((most * feature_tiles + 7) / 8 * 8)); };
-  if (wide)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true>), grid_of(d->inter / 128), dim3(256), 0, st, up);
-  else if (tile == 256)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 4, 2, 2, 4, false>), grid_of(d->inter / 128), dim3(512), 0, st, up);
-  else
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false>), grid_of(d->inter / 128), dim3(256), 0, st, up);
-  X8Args dn = up;
-  dn.x = up.h8;
-  dn.x_stride = d->inter;
-  dn.xs = up.hs;
-  dn.xs_stride = d->inter / kX8Block;
-  dn.w = static_cast<const uint8_t*>(d->w2);
-  dn.ws = d->w2_scale_inv;
-  dn.n = d->hidden;
-  dn.k = d->inter;
-  dn.y = at(l.slots);
-  dn.y_stride = d->hidden;
-  dn.y_dtype = d->out_dtype;
-  dn.vec = 1;
-  dn.pair_w = d->weights;
-  dn.pair_w_stride = d->weights_row_stride;
-  if (wide)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, true>), grid_of(d->hidden / 128), dim3(256), 0, st, dn);
-  else if (tile == 256)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 4, 2, 2, 4, false>), grid_of((d->hidden + 255) / 256), dim3(512), 0, st, dn);
-  else
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, false>), grid_of(d->hidden / 128), dim3(256), 0, st, dn);
+  if (kind == MoeKind::kFew) {
+    hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F32, false>), dim3(static_cast<unsigned>(most * (d->inter / 16))),
+                       dim3(256), 0, st, few);
+    hipLaunchKernelGGL(moe_down_few_kernel, dim3(static_cast<unsigned>(most * (d->hidden / 128))), dim3(256), 0, st, few);
+  } else {
+    launch_moe_tiles(*d, l, most, tile, st);
+  }
   const CombineArgs c{at(l.slots), d->ids, d->ids_row_stride, d->tokens, d->top_k, d->experts, d->hidden, d->out,
-                      d->out_row_stride, d->accumulate};
-  const dim3 grid(static_cast<unsigned>(((int64_t)d->tokens * (d->hidden / 4) + 255) / 256));
+                      d->out_row_stride, d->accumulate != 0,
+                      reinterpret_cast<uintptr_t>(d->out) % 16 == 0 && d->out_row_stride % 8 == 0};
+  const dim3 grid(static_cast<unsigned>(((int64_t)d->tokens * (d->hidden / 8) + 255) / 256));
   if (d->out_dtype == RIA_DT_BF16)
     hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_BF16>), grid, dim3(256), 0, st, c);
   else if (d->out_dtype == RIA_DT_F16)

@@ -50,6 +50,16 @@ __device__ __forceinline__ f32x16 mfma_x8_32(i32x8 a, i32x8 b, f32x16 c) {
   }
 }
 
+// 16x16 results over one block of K, both operands widened to fp16.
+__device__ __forceinline__ f32x4 mfma_x8_16(const u32x4 (&a)[2], const u32x4 (&b)[2]) {
+  f32x4 c{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    c = Kv16<RIA_DT_F16>::mfma_k32(x8_to_f16x8(a[i / 2][2 * (i % 2)], a[i / 2][2 * (i % 2) + 1]),
+                                   x8_to_f16x8(b[i / 2][2 * (i % 2)], b[i / 2][2 * (i % 2) + 1]), c);
+  return c;
+}
+
 __device__ __forceinline__ i32x8 join_x8(u32x4 lo, u32x4 hi) {
   return i32x8{static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
                static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
@@ -94,6 +104,13 @@ __device__ __forceinline__ float row16_max(float v) {
   v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x124, 0xf, 0xf, true)));  // row_ror:4
   v = fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xf, 0xf, true)));   // quad_perm
   return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xf, 0xf, true)));
+}
+
+// SiLU(g) u.  The hardware's exp2 and reciprocal are within an ulp; rounding -g
+// log2(e) before the exp2 adds |g| 2^-24 relative, 2^-20 where SiLU still
+// matters (g > -16): the e4m3 rounding that follows is 2^-4.
+__device__ __forceinline__ float x8_swiglu(float g, float u) {
+  return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
 }
 
 struct QuantArgs {
@@ -393,7 +410,7 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
       for (int f = 0; f < HF; ++f)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float v = silu_f(acc[f][t][i]) * acc[HF + f][t][i];
+          const float v = x8_swiglu(acc[f][t][i], acc[HF + f][t][i]);
           acc[f][t][i] = v;
           m = fmaxf(m, finite_abs(v));
         }
