@@ -367,31 +367,40 @@ struct FewArgs {
   int out_dtype, add;
 };
 
-// 16 rows of w at block kb of K: this lane's 32 bytes (row l % 16, part l / 16).
+// This lane's 32 bytes of a 128-byte row block: chunks l / 16 and l / 16 + 4 of
+// 16 bytes, so that one load takes 64 whole bytes of each of 16 rows.
+__device__ __forceinline__ void load_chunks(const uint8_t* row, int lane, u32x4 (&v)[2]) {
+  const u32x4* p = reinterpret_cast<const u32x4*>(row) + (lane >> 4);
+  v[0] = p[0];
+  v[1] = p[4];
+}
+// 16 rows of w at block kb of K (row l % 16 in this lane).
 __device__ __forceinline__ void load_rows16(const uint8_t* w, int k, int kb, int lane, u32x4 (&v)[2]) {
-  const u32x4* p = reinterpret_cast<const u32x4*>(w + (int64_t)(lane & 15) * k + kb * kX8Block + 32 * (lane >> 4));
-  v[0] = ld_stream(p);
-  v[1] = ld_stream(p + 1);
+  const u32x4* p = reinterpret_cast<const u32x4*>(w + (int64_t)(lane & 15) * k + kb * kX8Block) + (lane >> 4);
+  v[0] = p[0];
+  v[1] = p[4];
 }
 
-// act = SiLU(g) u of one tile and 16 features, four waves sharing K.  PAIRS:
-// the tile is one (token, slot) pair, and x is quantised here.
-template <int XT, bool PAIRS>
-__global__ __launch_bounds__(256) void moe_up_few_kernel(const FewArgs a) {
+// act = SiLU(g) u of one tile and 16 CG features, NW waves sharing K, each with
+// AH blocks of K in flight.  PAIRS: the tile is one (token, slot) pair, and x is
+// quantised here.
+template <int XT, bool PAIRS, int CG, int NW, int AH>
+__global__ __launch_bounds__(64 * NW) void moe_up_few_kernel(const FewArgs a) {
+  static_assert(64 * NW == 256 * CG, "a thread for each result of 16 rows");
   extern __shared__ __attribute__((aligned(16))) uint8_t xq_s[];  // PAIRS: hidden e4m3 values, then their scales
-  __shared__ f32x4 red[4][2][64];
+  __shared__ f32x4 red[NW][2 * CG][64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int groups = a.inter / 16;
-  const int tile = blockIdx.x / groups, c0 = blockIdx.x % groups * 16;
+  const int groups = a.inter / (16 * CG);
+  const int tile = blockIdx.x / groups, c0 = blockIdx.x % groups * 16 * CG;
   int expert, first, rows = 1;
   if constexpr (PAIRS) {
     first = tile;
     expert = a.ids[(int64_t)(tile / a.top_k) * a.id_stride + tile % a.top_k];
     if (expert < 0 || expert >= a.experts) return;
   } else {
+    const X8Tile t = a.tiles[tile];  // in step with the count: entries past it are allocated, and not used
     if (tile >= *a.ntiles) return;
-    const X8Tile t = a.tiles[tile];
     expert = t.expert;
     first = t.first;
     rows = t.rows;
@@ -404,24 +413,39 @@ __global__ __launch_bounds__(256) void moe_up_few_kernel(const FewArgs a) {
   const float* su = sg + (int64_t)(a.inter / kX8Block) * kblocks;
   const int at = first + min(lane & 15, rows - 1);
   const int64_t token = PAIRS ? tile / a.top_k : a.order[at] / a.top_k;
-  const uint8_t* x8 = a.x8 + token * k + 32 * (lane >> 4);
+  const uint8_t* x8 = a.x8 + token * k;
   const float* xs = a.xs + token * kblocks;
 
-  u32x4 g[kFewAhead][2], u[kFewAhead][2];
+  // a wave's blocks kb0 .. kb0 + AH - 1: weights first, so that no wait for them comes early
+  u32x4 w[AH][2 * CG][2], b[AH][2];
+  float fg[AH], fu[AH], fx[AH];
   auto load = [&](int kb0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kFewAhead; ++i) {
+    for (int i = 0; i < AH; ++i) {
       const int kb = min(kb0 + i, kblocks - 1);
-      load_rows16(wg, k, kb, lane, g[i]);
-      load_rows16(wu, k, kb, lane, u[i]);
+#pragma unroll
+      for (int c = 0; c < CG; ++c) {
+        load_rows16(wg + (int64_t)16 * c * k, k, kb, lane, w[i][c]);
+        load_rows16(wu + (int64_t)16 * c * k, k, kb, lane, w[i][CG + c]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < AH; ++i) {
+      const int kb = min(kb0 + i, kblocks - 1);
+      fg[i] = sg[kb];
+      fu[i] = su[kb];
+      if constexpr (!PAIRS) {
+        load_chunks(x8 + kb * kX8Block, lane, b[i]);
+        fx[i] = xs[kb];
+      }
     }
   };
-  load(wave * kFewAhead);
+  load(wave * AH);
   if constexpr (PAIRS) {
     uint8_t* q = xq_s;
     float* qs = reinterpret_cast<float*>(xq_s + k);
     const int64_t x0 = token * a.x_stride;
-    for (int c = 8 * tid; c < k; c += 8 * 256) {
+    for (int c = 8 * tid; c < k; c += 8 * 64 * NW) {
       float v[8];
       load_act8<XT>(a.x, x0 + c, v);
       float top = 0.f;
@@ -436,48 +460,41 @@ __global__ __launch_bounds__(256) void moe_up_few_kernel(const FewArgs a) {
     }
     lds_barrier();
   }
-  f32x4 ag{0.f, 0.f, 0.f, 0.f}, au = ag;
-  for (int kb0 = wave * kFewAhead; kb0 < kblocks; kb0 += 4 * kFewAhead) {
+  f32x4 acc[2 * CG];
 #pragma unroll
-    for (int i = 0; i < kFewAhead; ++i) {
+  for (int c = 0; c < 2 * CG; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int kb0 = wave * AH; kb0 < kblocks; kb0 += NW * AH) {
+#pragma unroll
+    for (int i = 0; i < AH; ++i) {
       const int kb = kb0 + i;
       if (kb >= kblocks) break;
-      u32x4 b[2];
-      float s;
       if constexpr (PAIRS) {
-        const u32x4* p = reinterpret_cast<const u32x4*>(xq_s + kb * kX8Block + 32 * (lane >> 4));
-        b[0] = p[0];
-        b[1] = p[1];
-        s = reinterpret_cast<const float*>(xq_s + k)[kb];
-      } else {
-        const u32x4* p = reinterpret_cast<const u32x4*>(x8 + kb * kX8Block);
-        b[0] = p[0];
-        b[1] = p[1];
-        s = xs[kb];
+        load_chunks(xq_s + kb * kX8Block, lane, b[i]);
+        fx[i] = reinterpret_cast<const float*>(xq_s + k)[kb];
       }
-      const f32x4 pg = mfma_x8_16(g[i], b), pu = mfma_x8_16(u[i], b);
-      const float fg = s * sg[kb], fu = s * su[kb];
+      const float s0 = fx[i] * fg[i], s1 = fx[i] * fu[i];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        ag[j] = fmaf(pg[j], fg, ag[j]);
-        au[j] = fmaf(pu[j], fu, au[j]);
+      for (int c = 0; c < 2 * CG; ++c) {
+        const f32x4 part = mfma_x8_16(w[i][c], b[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[c][j] = fmaf(part[j], c < CG ? s0 : s1, acc[c][j]);
       }
     }
-    if (kb0 + 4 * kFewAhead < kblocks) load(kb0 + 4 * kFewAhead);
+    if (kb0 + NW * AH < kblocks) load(kb0 + NW * AH);
   }
-  red[wave][0][lane] = ag;
-  red[wave][1][lane] = au;
+#pragma unroll
+  for (int c = 0; c < 2 * CG; ++c) red[wave][c][lane] = acc[c];
   __syncthreads();
-  // thread (row, feature): result (feature, row) of the products is value feature % 4 of lane row + 16 (feature / 4)
-  const int row = tid >> 4, f = tid & 15;
+  // thread (row, feature): result (feature, row) of a product is value feature % 4 of lane row + 16 (feature / 4)
+  const int row = tid / (16 * CG), f = tid % 16, c = tid / 16 % CG;
   if (row >= rows) return;
   float gate = 0.f, up = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    gate += red[w][0][row + 16 * (f >> 2)][f & 3];
-    up += red[w][1][row + 16 * (f >> 2)][f & 3];
+  for (int v = 0; v < NW; ++v) {
+    gate += red[v][c][row + 16 * (f >> 2)][f & 3];
+    up += red[v][CG + c][row + 16 * (f >> 2)][f & 3];
   }
-  a.act[(int64_t)(first + row) * a.inter + c0 + f] = x8_swiglu(gate, up);
+  a.act[(int64_t)(first + row) * a.inter + c0 + 16 * c + f] = x8_swiglu(gate, up);
 }
 
 // 8 values of act to e4m3 at d, their block's scale to s (16 lanes a block).
@@ -495,23 +512,24 @@ __device__ __forceinline__ void quant_act8(const float* p, uint8_t* d, float* s,
   if ((lane & 15) == 0) *s = x8_scale(e);
 }
 
-// One tile's rows of 128 features of the output (a wave: 32 of them), to the
+// One tile's rows of 32 NW features of the output (a wave: 32 of them), to the
 // pairs' slots.
-__global__ __launch_bounds__(256) void moe_down_few_kernel(const FewArgs a) {
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void moe_down_few_kernel(const FewArgs a) {
   constexpr int kPitch = kFewChunk + 16;  // 16 rows' reads meet all banks
   __shared__ __attribute__((aligned(16))) uint8_t h_s[kFewTile * kPitch];
   __shared__ float hs_s[kFewTile][kFewChunk / kX8Block];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int groups = a.hidden / 128;
+  const int groups = (a.hidden + 32 * NW - 1) / (32 * NW);
   const int tile = blockIdx.x / groups;
-  if (tile >= *a.ntiles) return;
   const X8Tile t = a.tiles[tile];
+  if (tile >= *a.ntiles) return;
   const int expert = __builtin_amdgcn_readfirstlane(t.expert), rows = __builtin_amdgcn_readfirstlane(t.rows);
-  const int n0 = blockIdx.x % groups * 128 + wave * 32;
+  const int n0 = min(blockIdx.x % groups * 32 * NW + wave * 32, a.hidden - 32);  // waves past the last feature repeat its group
   const int k = a.inter, kblocks = k / kX8Block;
   const uint8_t* w = a.w2 + ((int64_t)expert * a.hidden + n0) * k;
-  const float* s2 = a.s2 + ((int64_t)expert * groups + blockIdx.x % groups) * kblocks;
+  const float* s2 = a.s2 + ((int64_t)expert * (a.hidden / kX8Block) + n0 / kX8Block) * kblocks;
   u32x4 v[2][kFewAhead][2];
   auto load = [&](int kb0) __attribute__((always_inline)) {
 #pragma unroll
@@ -522,23 +540,25 @@ __global__ __launch_bounds__(256) void moe_down_few_kernel(const FewArgs a) {
     }
   };
   load(0);
+  const int row = min(lane & 15, rows - 1);
+  const int pair = a.order[t.first + row];  // ahead of the end, where its wait would show
+  const float pw = a.pair_w[(int64_t)(pair / a.top_k) * a.pair_w_stride + pair % a.top_k];
   f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
   for (int c0 = 0; c0 < k; c0 += kFewChunk) {
     const int cols = min(kFewChunk, k - c0), units = cols / 8;
     if (c0) __syncthreads();
-    for (int u = tid; u < rows * units; u += 256) {
+    for (int u = tid; u < rows * units; u += 64 * NW) {
       const int r = u / units, c = (u - r * units) * 8;
       quant_act8(a.act + (int64_t)(t.first + r) * k + c0 + c, h_s + r * kPitch + c, &hs_s[r][c / kX8Block], tid);
     }
     lds_barrier();
-    const int row = min(lane & 15, rows - 1);
     for (int b0 = 0; b0 < cols / kX8Block; b0 += kFewAhead) {
 #pragma unroll
       for (int i = 0; i < kFewAhead; ++i) {
         const int kb = b0 + i;  // of the chunk
         if (kb >= cols / kX8Block) break;
-        const u32x4* p = reinterpret_cast<const u32x4*>(h_s + row * kPitch + kb * kX8Block + 32 * (lane >> 4));
-        const u32x4 b[2] = {p[0], p[1]};
+        u32x4 b[2];
+        load_chunks(h_s + row * kPitch + kb * kX8Block, lane, b);
         const float s = hs_s[row][kb] * s2[c0 / kX8Block + kb];
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
@@ -552,11 +572,9 @@ __global__ __launch_bounds__(256) void moe_down_few_kernel(const FewArgs a) {
     }
   }
   if ((lane & 15) >= rows) return;
-  const int64_t pair = a.order[t.first + (lane & 15)];
-  const float pw = a.pair_w[pair / a.top_k * a.pair_w_stride + pair % a.top_k];
 #pragma unroll
   for (int f = 0; f < 2; ++f) {
-    const int64_t o = pair * a.hidden + n0 + 16 * f + 4 * (lane >> 4);
+    const int64_t o = (int64_t)pair * a.hidden + n0 + 16 * f + 4 * (lane >> 4);
     float r[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) r[j] = pw * acc[f][j];
@@ -607,8 +625,8 @@ __global__ __launch_bounds__(64 * kSumWaves) void moe_down_pairs_kernel(const Fe
           for (int i = 0; i < kFewAhead; ++i) {
             const int kb = b0 + i;
             if (kb >= cols / kX8Block) break;
-            const u32x4* p = reinterpret_cast<const u32x4*>(h_s[wave] + kb * kX8Block + 32 * (lane >> 4));
-            const u32x4 b[2] = {p[0], p[1]};
+            u32x4 b[2];
+            load_chunks(h_s[wave] + kb * kX8Block, lane, b);
             const float s = hs_s[wave][kb] * s2[c0 / kX8Block + kb];
             const f32x4 part = mfma_x8_16(v[i], b);
 #pragma unroll
@@ -879,11 +897,11 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
     const dim3 dgrid(static_cast<unsigned>((int64_t)d->tokens * (d->hidden / 16)));
     const size_t lds = d->hidden + d->hidden / kX8Block * 4;
     if (d->x_dtype == RIA_DT_BF16)
-      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_BF16, true>), ugrid, dim3(256), lds, st, few);
+      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_BF16, true, 1, 4, 4>), ugrid, dim3(256), lds, st, few);
     else if (d->x_dtype == RIA_DT_F16)
-      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F16, true>), ugrid, dim3(256), lds, st, few);
+      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F16, true, 1, 4, 4>), ugrid, dim3(256), lds, st, few);
     else
-      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F32, true>), ugrid, dim3(256), lds, st, few);
+      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F32, true, 1, 4, 4>), ugrid, dim3(256), lds, st, few);
     if (d->out_dtype == RIA_DT_BF16)
       hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_BF16>), dgrid, dim3(64 * kSumWaves), 0, st, few);
     else if (d->out_dtype == RIA_DT_F16)
@@ -906,9 +924,9 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
     hipLaunchKernelGGL((moe_prepare_kernel<RIA_DT_F32>), pgrid, dim3(256), 0, st, plan, quant);
   if (plan.blocks > 1) hipLaunchKernelGGL(moe_place_kernel, dim3(plan.blocks), dim3(256), 0, st, plan);
   if (kind == MoeKind::kFew) {
-    hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F32, false>), dim3(static_cast<unsigned>(most * (d->inter / 16))),
-                       dim3(256), 0, st, few);
-    hipLaunchKernelGGL(moe_down_few_kernel, dim3(static_cast<unsigned>(most * (d->hidden / 128))), dim3(256), 0, st, few);
+    hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F32, false, 2, 8, 2>), dim3(static_cast<unsigned>(most * (d->inter / 32))),
+                       dim3(512), 0, st, few);
+    hipLaunchKernelGGL((moe_down_few_kernel<4>), dim3(static_cast<unsigned>(most * (d->hidden / 128))), dim3(256), 0, st, few);
   } else {
     launch_moe_tiles(*d, l, most, tile, st);
   }

@@ -1146,25 +1146,34 @@ _SCORING = {"softmax": nat.RIA_ROUTE_SOFTMAX, "sigmoid": nat.RIA_ROUTE_SIGMOID}
 _GROUP_SCORE = {"max": nat.RIA_ROUTE_GROUP_MAX, "top2": nat.RIA_ROUTE_GROUP_TOP2}
 
 
-def _call(name: str, dev: torch.device, *args) -> None:
-    """One entry point on the current stream of `dev`, which is made the current device for it."""
-    fn = getattr(nat.load(), name)
-    index = dev.index
-    if index is None or index == torch.cuda.current_device():
-        rc = fn(*args, _stream(dev))
+# The calls below are shorter on the GPU than on the host for small batches: as
+# above, they compare plain ints and take the slow path only to say what is wrong.
+def _same_device(named: dict[str, torch.Tensor | None]) -> None:
+    """The error of tensors that are not all on the first one's GPU."""
+    first = next(iter(named.values()))
+    for name, t in named.items():
+        _require_gpu(name, t, first.device if first.is_cuda else None)
+
+
+def _run(fn, name: str, index: int, *args) -> None:
+    """One entry point on the current stream of GPU `index`, which is made the current device for it."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _stream(dev))
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         nat.check(rc, name)
 
 
-def _rows_2d(name: str, t: torch.Tensor, cols: int) -> int:
-    """Row stride (elements) of a 2-D tensor with `cols` contiguous columns."""
-    if t.dim() != 2 or t.shape[1] != cols or (cols > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} must be [rows, {cols}] with contiguous rows, got {tuple(t.shape)} "
-                         f"strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else cols
+def _rows_2d(name: str, t: torch.Tensor, rows: int, cols: int) -> int:
+    """Row stride (elements) of a [rows, cols] tensor whose columns are contiguous."""
+    if t.is_contiguous():
+        if t.shape == (rows, cols):
+            return cols
+    elif t.shape == (rows, cols) and (cols == 1 or t.stride(1) == 1):
+        return t.stride(0) if rows > 1 else cols
+    raise ValueError(f"{name} must be [{rows}, {cols}] with contiguous rows, got {tuple(t.shape)} strides {t.stride()}")
 
 
 def quant_fp8(x: torch.Tensor, *, out: torch.Tensor | None = None,
@@ -1175,27 +1184,29 @@ def quant_fp8(x: torch.Tensor, *, out: torch.Tensor | None = None,
     [M, K] float8_e4m3fn, scale [M, K / 128] fp32) with x ~ x8 * scale: the
     scale is the smallest power of two with |x8| <= 448.
     """
-    dev = x.device
-    _require_gpu("x", x)
+    index = x.get_device()
+    if index < 0:
+        _require_gpu("x", x)
     if x.dim() != 2:
         raise ValueError(f"x must be [M, K], got {tuple(x.shape)}")
     m, k = x.shape
     if k == 0 or k % FP8_BLOCK:
         raise ValueError(f"x must have a multiple of {FP8_BLOCK} columns, got {k}")
-    xs = _rows_2d("x", x, k)
+    blocks = k // FP8_BLOCK
+    xs = _rows_2d("x", x, m, k)
     if out is None:
-        out = torch.empty((m, k), dtype=torch.float8_e4m3fn, device=dev)
-    else:
-        _require_gpu("out", out, dev)
-        if out.dtype not in _E4M3 or out.shape != (m, k) or not out.is_contiguous():
-            raise ValueError(f"out must be contiguous float8_e4m3fn [{m}, {k}]")
+        out = torch.empty(m, k, dtype=torch.float8_e4m3fn, device=x.device)
+    elif out.get_device() != index or out.dtype not in _E4M3 or out.shape != (m, k) or not out.is_contiguous():
+        _require_gpu("out", out, x.device)
+        raise ValueError(f"out must be contiguous float8_e4m3fn [{m}, {k}]")
     if scale is None:
-        scale = torch.empty((m, k // FP8_BLOCK), dtype=torch.float32, device=dev)
-    else:
-        _require_gpu("scale", scale, dev)
-        if scale.dtype != torch.float32 or scale.shape != (m, k // FP8_BLOCK) or not scale.is_contiguous():
-            raise ValueError(f"scale must be contiguous fp32 [{m}, {k // FP8_BLOCK}]")
-    _call("ria_quant_fp8", dev, m, k, x.data_ptr(), dtype_code(x), xs, out.data_ptr(), scale.data_ptr())
+        scale = torch.empty(m, blocks, dtype=torch.float32, device=x.device)
+    elif scale.get_device() != index or scale.dtype != torch.float32 or scale.shape != (m, blocks) \
+            or not scale.is_contiguous():
+        _require_gpu("scale", scale, x.device)
+        raise ValueError(f"scale must be contiguous fp32 [{m}, {blocks}]")
+    _run(nat.load().ria_quant_fp8, "ria_quant_fp8", index, m, k, x.data_ptr(), dtype_code(x), xs, out.data_ptr(),
+         scale.data_ptr())
     return out, scale
 
 
@@ -1209,31 +1220,29 @@ def linear_fp8_x8(x8: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor,
     scales, as linear_fp8 takes them.  Returns / fills y [M, N]; with
     ``accumulate`` the fp32 ``out`` receives out + y.
     """
-    dev = x8.device
-    _require_gpu("x8", x8)
-    _require_gpu("x_scale", x_scale, dev)
-    n, k = _fp8_weight("weight", weight, scale_inv, dev)
+    index = x8.get_device()
+    if index < 0 or not index == x_scale.get_device() == weight.get_device() == scale_inv.get_device():
+        _same_device({"x8": x8, "x_scale": x_scale, "weight": weight, "weight scale_inv": scale_inv})
+    n, k = _fp8_weight("weight", weight, scale_inv, x8.device)
     if x8.dtype not in _E4M3:
         raise ValueError(f"x8 must be float8_e4m3fn (or its uint8 bytes), got {x8.dtype}")
-    xs = _rows_2d("x8", x8, k)
-    m = x8.shape[0]
-    if x_scale.dtype != torch.float32 or x_scale.shape[0] != m:
-        raise ValueError(f"x_scale must be fp32 [{m}, {k // FP8_BLOCK}], got {x_scale.dtype} {tuple(x_scale.shape)}")
-    ss = _rows_2d("x_scale", x_scale, k // FP8_BLOCK)
+    m = x8.shape[0] if x8.dim() == 2 else -1
+    xs = _rows_2d("x8", x8, m, k)
+    if x_scale.dtype != torch.float32:
+        raise ValueError(f"x_scale must be fp32 [{m}, {k // FP8_BLOCK}], got {x_scale.dtype}")
+    ss = _rows_2d("x_scale", x_scale, m, k // FP8_BLOCK)
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty((m, n), dtype=out_dtype, device=dev)
+        out = torch.empty(m, n, dtype=out_dtype, device=x8.device)
         ys = n
     else:
-        _require_gpu("out", out, dev)
-        ys = _rows_2d("out", out, n)
-        if out.shape[0] != m:
-            raise ValueError(f"out must have {m} rows, got {out.shape[0]}")
+        _require_gpu("out", out, x8.device)
+        ys = _rows_2d("out", out, m, n)
         if accumulate and out.dtype != torch.float32:
             raise ValueError("accumulate needs an fp32 out")
-    _call("ria_linear_fp8_x8", dev, m, n, k, x8.data_ptr(), xs, x_scale.data_ptr(), ss, weight.data_ptr(),
-          scale_inv.data_ptr(), out.data_ptr(), dtype_code(out), ys, int(accumulate))
+    _run(nat.load().ria_linear_fp8_x8, "ria_linear_fp8_x8", index, m, n, k, x8.data_ptr(), xs, x_scale.data_ptr(), ss,
+         weight.data_ptr(), scale_inv.data_ptr(), out.data_ptr(), dtype_code(out), ys, bool(accumulate))
     return out
 
 
@@ -1254,54 +1263,58 @@ def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bia
     last the gate of an expert that every token visits: slot k is (sigmoid of
     it, E).
     """
-    dev = logits.device
-    _require_gpu("logits", logits)
+    index = logits.get_device()
+    if index < 0:
+        _require_gpu("logits", logits)
     s = 1 if shared_expert else 0
     if logits.dim() != 2 or logits.shape[1] <= s:
         raise ValueError(f"logits must be [tokens, experts{' + 1' if s else ''}], got {tuple(logits.shape)}")
     t, cols = logits.shape
     e = cols - s
-    ls = _rows_2d("logits", logits, cols)
+    ls = _rows_2d("logits", logits, t, cols)
     if scoring not in _SCORING or group_score not in _GROUP_SCORE:
         raise ValueError(f"scoring must be one of {sorted(_SCORING)}, group_score one of {sorted(_GROUP_SCORE)}")
-    if bias is not None:
-        _require_gpu("bias", bias, dev)
-        if bias.dtype != torch.float32 or bias.shape != (e,) or not bias.is_contiguous():
-            raise ValueError(f"bias must be contiguous fp32 [{e}]")
-    width = top_k + s
+    if bias is not None and (bias.get_device() != index or bias.dtype != torch.float32 or bias.shape != (e,)
+                             or not bias.is_contiguous()):
+        _require_gpu("bias", bias, logits.device)
+        raise ValueError(f"bias must be contiguous fp32 [{e}]")
+    width = ws = ds = top_k + s
+    if not 1 <= top_k <= e:
+        raise ValueError(f"top_k must be 1 to the number of experts ({e}), got {top_k}")
     if weights is None:
-        weights = torch.empty((t, width), dtype=torch.float32, device=dev)
+        weights = torch.empty(t, width, dtype=torch.float32, device=logits.device)
+    else:
+        _require_gpu("weights", weights, logits.device)
+        ws = _rows_2d("weights", weights, t, width)
     if ids is None:
-        ids = torch.empty((t, width), dtype=torch.int32, device=dev)
-    _require_gpu("weights", weights, dev)
-    _require_gpu("ids", ids, dev)
-    ws, ds = _rows_2d("weights", weights, width), _rows_2d("ids", ids, width)
-    if weights.dtype != torch.float32 or ids.dtype != torch.int32 or weights.shape[0] != t or ids.shape[0] != t:
-        raise ValueError(f"weights must be fp32 and ids int32, both [{t}, {width}]")
-    _call("ria_moe_route", dev, t, e, top_k, logits.data_ptr(), dtype_code(logits), ls, _SCORING[scoring], _ptr(bias),
-          num_groups, top_groups, _GROUP_SCORE[group_score], int(renormalize), scale, s, weights.data_ptr(), ws,
-          ids.data_ptr(), ds)
+        ids = torch.empty(t, width, dtype=torch.int32, device=logits.device)
+    else:
+        _require_gpu("ids", ids, logits.device)
+        ds = _rows_2d("ids", ids, t, width)
+    if weights.dtype != torch.float32 or ids.dtype != torch.int32:
+        raise ValueError(f"weights must be fp32 and ids int32, got {weights.dtype} and {ids.dtype}")
+    _run(nat.load().ria_moe_route, "ria_moe_route", index, t, e, top_k, logits.data_ptr(), dtype_code(logits), ls,
+         _SCORING[scoring], _ptr(bias), num_groups, top_groups, _GROUP_SCORE[group_score], bool(renormalize), scale, s,
+         weights.data_ptr(), ws, ids.data_ptr(), ds)
     return weights, ids
 
 
 def moe_experts_workspace_bytes(tokens: int, top_k: int, experts: int, hidden: int, inter: int,
                                 out_dtype: torch.dtype = torch.float16) -> int:
     """Bytes of the workspace moe_experts takes for these sizes (ria_moe_experts_workspace_bytes)."""
-    n = int(nat.load().ria_moe_experts_workspace_bytes(tokens, top_k, experts, hidden, inter, _DTYPE_CODE[out_dtype]))
+    n = nat.load().ria_moe_experts_workspace_bytes(tokens, top_k, experts, hidden, inter, _DTYPE_CODE[out_dtype])
     if n < 0:
         raise ValueError(f"sizes refused: {tokens} tokens x {top_k} of {experts} experts, hidden {hidden}, inter {inter}")
     return n
 
 
-def _expert_weight(name: str, w: torch.Tensor, scale_inv: torch.Tensor, shape: tuple[int, int, int],
-                   dev: torch.device) -> None:
-    _require_gpu(name, w, dev)
-    _require_gpu(name + " scale_inv", scale_inv, dev)
-    if w.dtype not in _E4M3 or w.shape != shape or not w.is_contiguous():
-        raise ValueError(f"{name} must be contiguous float8_e4m3fn {list(shape)}, got {w.dtype} {tuple(w.shape)}")
-    grid = (shape[0], shape[1] // FP8_BLOCK, shape[2] // FP8_BLOCK)
-    if scale_inv.dtype != torch.float32 or scale_inv.shape != grid or not scale_inv.is_contiguous():
-        raise ValueError(f"{name} scale_inv must be contiguous fp32 {list(grid)}, got {tuple(scale_inv.shape)}")
+def _expert_weight(name: str, w: torch.Tensor, scale_inv: torch.Tensor, e: int, n: int, k: int) -> None:
+    if w.dtype not in _E4M3 or w.shape != (e, n, k) or not w.is_contiguous():
+        raise ValueError(f"{name} must be contiguous float8_e4m3fn {[e, n, k]}, got {w.dtype} {tuple(w.shape)}")
+    if scale_inv.dtype != torch.float32 or scale_inv.shape != (e, n // FP8_BLOCK, k // FP8_BLOCK) \
+            or not scale_inv.is_contiguous():
+        raise ValueError(f"{name} scale_inv must be contiguous fp32 {[e, n // FP8_BLOCK, k // FP8_BLOCK]}, "
+                         f"got {tuple(scale_inv.shape)}")
 
 
 def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: torch.Tensor, s13: torch.Tensor,
@@ -1320,45 +1333,42 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: 
     ``workspace``: uint8, moe_experts_workspace_bytes (allocated if not given);
     calls that may overlap need one each.
     """
-    dev = x.device
-    _require_gpu("x", x)
-    if x.dim() != 2 or w13.dim() != 3 or w2.dim() != 3:
-        raise ValueError("x must be [T, H], w13 [E, 2 I, H] and w2 [E, H, I]")
+    index = x.get_device()
+    if index < 0 or not (index == ids.get_device() == weights.get_device() == w13.get_device() == s13.get_device()
+                         == w2.get_device() == s2.get_device()):
+        _same_device({"x": x, "ids": ids, "weights": weights, "w13": w13, "w13 scale_inv": s13, "w2": w2,
+                      "w2 scale_inv": s2})
+    if x.dim() != 2 or w13.dim() != 3 or w2.dim() != 3 or ids.dim() != 2:
+        raise ValueError("x must be [T, H], ids [T, k], w13 [E, 2 I, H] and w2 [E, H, I]")
     t, h = x.shape
-    e, i = w13.shape[0], w2.shape[2]
+    e, _, i = w2.shape
+    k = ids.shape[1]
     if e < 1 or h == 0 or i == 0 or h % FP8_BLOCK or i % FP8_BLOCK:
         raise ValueError(f"hidden {h} and inter {i} must be positive multiples of {FP8_BLOCK}, with 1 expert or more")
-    xs = _rows_2d("x", x, h)
-    _expert_weight("w13", w13, s13, (e, 2 * i, h), dev)
-    _expert_weight("w2", w2, s2, (e, h, i), dev)
-    _require_gpu("ids", ids, dev)
-    _require_gpu("weights", weights, dev)
-    if ids.dim() != 2 or ids.shape[0] != t or ids.shape[1] < 1 or ids.dtype != torch.int32 \
-            or weights.shape != ids.shape or weights.dtype != torch.float32:
-        raise ValueError(f"ids must be int32 and weights fp32, both [{t}, k], got {ids.dtype} {tuple(ids.shape)} and "
-                         f"{weights.dtype} {tuple(weights.shape)}")
-    k = ids.shape[1]
-    ds, ws = _rows_2d("ids", ids, k), _rows_2d("weights", weights, k)
+    _expert_weight("w13", w13, s13, e, 2 * i, h)
+    _expert_weight("w2", w2, s2, e, h, i)
+    xs, ds, ws = _rows_2d("x", x, t, h), _rows_2d("ids", ids, t, k), _rows_2d("weights", weights, t, k)
+    if k < 1 or ids.dtype != torch.int32 or weights.dtype != torch.float32:
+        raise ValueError(f"ids must be int32 and weights fp32, both [{t}, k], got {ids.dtype} and {weights.dtype}")
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty((t, h), dtype=out_dtype or x.dtype, device=dev)
+        out = torch.empty(t, h, dtype=out_dtype or x.dtype, device=x.device)
         os_ = h
     else:
-        _require_gpu("out", out, dev)
-        os_ = _rows_2d("out", out, h)
-        if out.shape[0] != t:
-            raise ValueError(f"out must have {t} rows, got {out.shape[0]}")
+        _require_gpu("out", out, x.device)
+        os_ = _rows_2d("out", out, t, h)
         if accumulate and out.dtype != torch.float32:
             raise ValueError("accumulate needs an fp32 out")
     if workspace is None:
-        workspace = torch.empty(moe_experts_workspace_bytes(t, k, e, h, i, out.dtype), dtype=torch.uint8, device=dev)
+        workspace = torch.empty(moe_experts_workspace_bytes(t, k, e, h, i, out.dtype), dtype=torch.uint8,
+                                device=x.device)
     else:
-        _require_gpu("workspace", workspace, dev)
+        _require_gpu("workspace", workspace, x.device)
         if not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
     d = nat.MoeExpertsDesc(t, k, e, h, i, x.data_ptr(), dtype_code(x), xs, ids.data_ptr(), ds, weights.data_ptr(), ws,
                            w13.data_ptr(), s13.data_ptr(), w2.data_ptr(), s2.data_ptr(), out.data_ptr(),
-                           dtype_code(out), os_, int(accumulate), workspace.data_ptr(), workspace.nbytes)
-    _call("ria_moe_experts", dev, ctypes.addressof(d))
+                           dtype_code(out), os_, bool(accumulate), workspace.data_ptr(), workspace.nbytes)
+    _run(nat.load().ria_moe_experts, "ria_moe_experts", index, ctypes.addressof(d))
     return out
