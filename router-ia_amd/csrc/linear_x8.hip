@@ -18,6 +18,200 @@ __global__ __launch_bounds__(256) void quant_fp8_kernel(const QuantArgs a) {
   quant_unit<XT>(a, (int64_t)blockIdx.x * 256 + threadIdx.x);
 }
 
+// A few rows: 16 features x up to 16 MT rows a workgroup, NW waves sharing K.
+// The weights stream from HBM straight into MFMA operands (16 rows x 128 bytes a
+// product, widened to fp16), all of a wave's kFewAhead blocks in flight at once.
+constexpr int kFewAhead = 4;
+template <int MT, int NW>
+__global__ __launch_bounds__(64 * NW) void x8_few_kernel(const X8Args a) {
+  __shared__ f32x4 red[NW][MT][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+  const int rows = min(16 * MT, a.m - m0);
+  const int kblocks = a.k / kX8Block;
+  const uint8_t* w = a.w + (int64_t)n0 * a.k;
+  const float* ws = a.ws + (int64_t)(n0 / kX8Block) * kblocks;
+  const uint8_t* x[MT];
+  const float* xs[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {  // rows past the last repeat it: computed, never stored
+    const int64_t row = m0 + min(16 * t + (lane & 15), rows - 1);
+    x[t] = a.x + row * a.x_stride;
+    xs[t] = a.xs + row * a.xs_stride;
+  }
+  u32x4 v[kFewAhead][2], b[kFewAhead][MT][2];
+  float fw[kFewAhead], fx[kFewAhead][MT];
+  auto load = [&](int kb0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) load_rows16(w, a.k, min(kb0 + i, kblocks - 1), lane, v[i]);
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int kb = min(kb0 + i, kblocks - 1);
+      fw[i] = ws[kb];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        load_chunks(x[t] + kb * kX8Block, lane, b[i][t]);
+        fx[i][t] = xs[t][kb];
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // all of them in flight before the first product
+  };
+  load(wave * kFewAhead);
+  f32x4 acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int kb0 = wave * kFewAhead; kb0 < kblocks; kb0 += NW * kFewAhead) {
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      if (kb0 + i >= kblocks) break;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const f32x4 part = mfma_x8_16(v[i], b[i][t]);
+        const float s = fx[i][t] * fw[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[t][j] = fmaf(part[j], s, acc[t][j]);
+      }
+    }
+    if (kb0 + NW * kFewAhead < kblocks) load(kb0 + NW * kFewAhead);
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) red[wave][t][lane] = acc[t];
+  __syncthreads();
+  // lane l of a product: row l % 16, features 4 (l / 16) .. + 3
+  for (int u = tid; u < 64 * MT; u += 64 * NW) {
+    const int t = u >> 6, l = ((u & 3) << 4) | ((u >> 2) & 15);  // neighbours in a row are neighbours here
+    const int row = 16 * t + (l & 15);
+    if (row >= rows) continue;
+    f32x4 s = red[0][t][l];
+#pragma unroll
+    for (int j = 1; j < NW; ++j) s += red[j][t][l];
+    store_four(a, (int64_t)(m0 + row) * a.y_stride + n0 + 4 * (l >> 4), s);
+  }
+}
+
+// Some hundred rows: 64 x 64 tiles, the blocks of K dealt to the workgroup's
+// four waves.  Each wave copies its blocks into two halves of LDS of its own
+// and multiplies them with no barrier; the four sums meet in LDS at the end.
+constexpr int kDealWaves = 4;
+template <bool WIDE>
+__global__ __launch_bounds__(64 * kDealWaves) void x8_deal_kernel(const X8Args a) {
+  constexpr int kStep = 128 * kX8Block;  // 64 rows of w, 64 of x
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kDealWaves * 2 * kStep];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, half = lane >> 5;
+  const int ntn = (a.n + 63) / 64, ntm = (a.m + 63) / 64;
+  const int at = x8_order(blockIdx.x, ntn * ntm);
+  if (at >= ntn * ntm) return;
+  const int n0 = at / ntm * 64, m0 = at % ntm * 64;  // neighbours share their weights
+  const int rows = min(64, a.m - m0), feats = min(64, a.n - n0);
+  const int kblocks = a.k / kX8Block;
+  const __amdgpu_buffer_rsrc_t wr = x8_rsrc(a.w + (int64_t)n0 * a.k, (int64_t)feats * a.k);
+  const __amdgpu_buffer_rsrc_t xr = x8_rsrc(a.x + m0 * a.x_stride, (rows - 1) * a.x_stride + a.k);
+  uint32_t wo[8], xo[8];  // rows past the last repeat it
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 8 * i + (lane >> 3), c = 16 * ((lane & 7) ^ ((r >> 1) & 7));
+    wo[i] = static_cast<uint32_t>(min(r, feats - 1)) * a.k + c;
+    xo[i] = static_cast<uint32_t>(min(r, rows - 1) * a.x_stride) + c;
+  }
+  const __amdgpu_buffer_rsrc_t xsr = x8_rsrc_f32(a.xs + m0 * a.xs_stride, (rows - 1) * a.xs_stride + kblocks);
+  const __amdgpu_buffer_rsrc_t wsr = x8_rsrc_f32(a.ws + (int64_t)(n0 / kX8Block) * kblocks, kblocks);
+  uint32_t xso[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) xso[t] = static_cast<uint32_t>(4 * min(32 * t + l32, rows - 1) * a.xs_stride);
+  uint8_t* own = lds + wave * 2 * kStep;
+  float xs[2][2], sw[2];
+  constexpr int kIssued = 3 + 16;
+  auto issue = [&](int kb, int h) __attribute__((always_inline)) {  // kIssued vector-memory loads
+    xs[h][0] = x8_load_f32(xsr, xso[0], 4 * kb);
+    xs[h][1] = x8_load_f32(xsr, xso[1], 4 * kb);
+    sw[h] = x8_load_f32(wsr, 0, 4 * kb);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x8_copy(wr, own + h * kStep + i * 1024, wo[i], kb * kX8Block);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x8_copy(xr, own + h * kStep + (8 + i) * 1024, xo[i], kb * kX8Block);
+  };
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int f = 0; f < 2; ++f)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[f][t][i] = 0.f;
+  auto operand = [&](const uint8_t* base, int r, int s) __attribute__((always_inline)) {
+    const int z = (r >> 1) & 7, c = 4 * s + 2 * half;
+    return join_x8(*reinterpret_cast<const u32x4*>(base + r * kX8Block + 16 * (c ^ z)),
+                   *reinterpret_cast<const u32x4*>(base + r * kX8Block + 16 * ((c + 1) ^ z)));
+  };
+  auto step = [&](int h) __attribute__((always_inline)) {
+    const uint8_t* d = own + h * kStep;
+    i32x8 b[2][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) b[t][s] = operand(d + 64 * kX8Block, 32 * t + l32, s);
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const i32x8 a0 = operand(d, 32 * f + l32, 0), a1 = operand(d, 32 * f + l32, 1);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x16 part;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[i] = 0.f;
+        part = mfma_x8_32<WIDE>(a0, b[t][0], part);
+        part = mfma_x8_32<WIDE>(a1, b[t][1], part);
+        const float sc = xs[h][t] * sw[h];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[f][t][i] = fmaf(part[i], sc, acc[f][t][i]);
+      }
+    }
+  };
+  // two blocks a turn, so that the halves are compile-time
+  if (wave < kblocks) {
+    issue(wave, 0);
+    for (int kb = wave; kb < kblocks; kb += 2 * kDealWaves) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (kb + h * kDealWaves >= kblocks) break;
+        const int next = kb + (h + 1) * kDealWaves;
+        if (next < kblocks) {
+          issue(next, h ^ 1);
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kIssued) : "memory");  // all but the loads just issued
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        step(h);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this half is read before it is copied to again
+      }
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  // sums [wave][row of x][64 features], chunks of four swizzled
+  f32x4* sum = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = 32 * t + l32;
+        sum[(wave * 64 + r) * 16 + ((8 * f + 2 * q + half) ^ (r & 15))] =
+            f32x4{acc[f][t][4 * q], acc[f][t][4 * q + 1], acc[f][t][4 * q + 2], acc[f][t][4 * q + 3]};
+      }
+  __syncthreads();
+  for (int u = tid; u < 64 * 16; u += 64 * kDealWaves) {
+    const int r = u >> 4, c = u & 15, at_c = c ^ (r & 15);
+    if (r >= rows || n0 + 4 * c >= a.n) continue;
+    f32x4 s = sum[r * 16 + at_c];
+#pragma unroll
+    for (int j = 1; j < kDealWaves; ++j) s += sum[(j * 64 + r) * 16 + at_c];
+    store_four(a, (int64_t)(m0 + r) * a.y_stride + n0 + 4 * c, s);
+  }
+}
+
 bool x8_dtype_ok(int dt) { return dt == RIA_DT_BF16 || dt == RIA_DT_F16 || dt == RIA_DT_F32; }
 
 }  // namespace ria
@@ -62,6 +256,7 @@ extern "C" int ria_linear_fp8_x8(int m, int n, int k, const void* x, int64_t x_r
   if (!x || !x_scale || !weight || !scale_inv || !y) return set_error(RIA_ERR_INVALID, "%s: null pointer", who);
   if (x_row_stride < k || x_row_stride % 16 || reinterpret_cast<uintptr_t>(x) % 16)
     return set_error(RIA_ERR_INVALID, "%s: x must be 16-byte aligned with a row stride of at least K, a multiple of 16", who);
+  if (x_scale_row_stride > (1 << 23)) return set_error(RIA_ERR_INVALID, "%s: x_scale row stride over 2^23", who);
   if (x_scale_row_stride < k / kX8Block) return set_error(RIA_ERR_INVALID, "%s: x_scale row stride too small", who);
   if (y_row_stride < n) return set_error(RIA_ERR_INVALID, "%s: y row stride too small", who);
   if (reinterpret_cast<uintptr_t>(weight) % 16) return set_error(RIA_ERR_INVALID, "%s: weight must be 16-byte aligned", who);
@@ -83,13 +278,36 @@ extern "C" int ria_linear_fp8_x8(int m, int n, int k, const void* x, int64_t x_r
   if (x_row_stride > (1 << 23)) return set_error(RIA_ERR_INVALID, "%s: x row stride over 8 MiB", who);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t t256 = (int64_t)((m + 255) / 256) * ((n + 255) / 256), t128 = (int64_t)((m + 127) / 128) * ((n + 127) / 128);
-  if (t128 > 0x7ffffff0) return set_error(RIA_ERR_INVALID, "%s: too many rows", who);
-  const dim3 g256(static_cast<unsigned>((t256 + 7) / 8 * 8)), g128(static_cast<unsigned>((t128 + 7) / 8 * 8));
-  if (y_dtype == RIA_DT_F32)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, true>), g128, dim3(256), 0, st, a);
-  else if (t256 >= 256)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 4, 2, 2, 4, false>), g256, dim3(512), 0, st, a);
-  else
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, false>), g128, dim3(256), 0, st, a);
+  const int64_t t64 = (int64_t)((m + 63) / 64) * ((n + 63) / 64);
+  if (t64 > 0x7ffffff0) return set_error(RIA_ERR_INVALID, "%s: too many rows", who);
+  auto grid = [](int64_t tiles) { return dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)); };
+  const bool wide = y_dtype == RIA_DT_F32;
+  if (m <= 64) {
+    const int mt = m <= 16 ? 1 : m <= 32 ? 2 : 4;
+    const dim3 few(n / 16, 1);
+    const bool deep = k > 2048;  // blocks of K past 4 waves x kFewAhead
+    if (mt == 1 && deep)
+      hipLaunchKernelGGL((x8_few_kernel<1, 8>), few, dim3(512), 0, st, a);
+    else if (mt == 1)
+      hipLaunchKernelGGL((x8_few_kernel<1, 4>), few, dim3(256), 0, st, a);
+    else if (mt == 2 && deep)
+      hipLaunchKernelGGL((x8_few_kernel<2, 8>), few, dim3(512), 0, st, a);
+    else if (mt == 2)
+      hipLaunchKernelGGL((x8_few_kernel<2, 4>), few, dim3(256), 0, st, a);
+    else if (deep)
+      hipLaunchKernelGGL((x8_few_kernel<4, 8>), few, dim3(512), 0, st, a);
+    else
+      hipLaunchKernelGGL((x8_few_kernel<4, 4>), few, dim3(256), 0, st, a);
+  } else if (t256 >= 192 && !wide) {
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 4, 2, 2, 4, false>), grid(t256), dim3(512), 0, st, a);
+  } else if (t128 >= 512 && !wide) {
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, false>), grid(t128), dim3(256), 0, st, a);
+  } else if (t128 >= 512) {
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, true>), grid(t128), dim3(256), 0, st, a);
+  } else if (!wide) {
+    hipLaunchKernelGGL((x8_deal_kernel<false>), grid(t64), dim3(64 * kDealWaves), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((x8_deal_kernel<true>), grid(t64), dim3(64 * kDealWaves), 0, st, a);
+  }
   return check_launch(who);
 }

@@ -367,20 +367,6 @@ struct FewArgs {
   int out_dtype, add;
 };
 
-// This lane's 32 bytes of a 128-byte row block: chunks l / 16 and l / 16 + 4 of
-// 16 bytes, so that one load takes 64 whole bytes of each of 16 rows.
-__device__ __forceinline__ void load_chunks(const uint8_t* row, int lane, u32x4 (&v)[2]) {
-  const u32x4* p = reinterpret_cast<const u32x4*>(row) + (lane >> 4);
-  v[0] = p[0];
-  v[1] = p[4];
-}
-// 16 rows of w at block kb of K (row l % 16 in this lane).
-__device__ __forceinline__ void load_rows16(const uint8_t* w, int k, int kb, int lane, u32x4 (&v)[2]) {
-  const u32x4* p = reinterpret_cast<const u32x4*>(w + (int64_t)(lane & 15) * k + kb * kX8Block) + (lane >> 4);
-  v[0] = p[0];
-  v[1] = p[4];
-}
-
 // act = SiLU(g) u of one tile and 16 CG features, NW waves sharing K, each with
 // AH blocks of K in flight.  PAIRS: the tile is one (token, slot) pair, and x is
 // quantised here.
@@ -439,6 +425,7 @@ __global__ __launch_bounds__(64 * NW) void moe_up_few_kernel(const FewArgs a) {
         fx[i] = xs[kb];
       }
     }
+    __builtin_amdgcn_sched_barrier(0);  // all of them in flight before the first product
   };
   load(wave * AH);
   if constexpr (PAIRS) {

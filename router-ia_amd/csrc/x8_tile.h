@@ -60,6 +60,20 @@ __device__ __forceinline__ f32x4 mfma_x8_16(const u32x4 (&a)[2], const u32x4 (&b
   return c;
 }
 
+// This lane's 32 bytes of a 128-byte row block: chunks l / 16 and l / 16 + 4 of
+// 16 bytes, so that one load takes 64 whole bytes of each of 16 rows.
+__device__ __forceinline__ void load_chunks(const uint8_t* row, int lane, u32x4 (&v)[2]) {
+  const u32x4* p = reinterpret_cast<const u32x4*>(row) + (lane >> 4);
+  v[0] = p[0];
+  v[1] = p[4];
+}
+// 16 rows of w at block kb of K (row l % 16 in this lane).
+__device__ __forceinline__ void load_rows16(const uint8_t* w, int k, int kb, int lane, u32x4 (&v)[2]) {
+  const u32x4* p = reinterpret_cast<const u32x4*>(w + (int64_t)(lane & 15) * k + kb * kX8Block) + (lane >> 4);
+  v[0] = p[0];
+  v[1] = p[4];
+}
+
 __device__ __forceinline__ i32x8 join_x8(u32x4 lo, u32x4 hi) {
   return i32x8{static_cast<int>(lo[0]), static_cast<int>(lo[1]), static_cast<int>(lo[2]), static_cast<int>(lo[3]),
                static_cast<int>(hi[0]), static_cast<int>(hi[1]), static_cast<int>(hi[2]), static_cast<int>(hi[3])};
@@ -184,6 +198,36 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t x8_rsrc(const uint8_t* p, int6
 }
 __device__ __forceinline__ void x8_copy(__amdgpu_buffer_rsrc_t r, uint8_t* d, uint32_t lane_offset, int offset) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, d, 16, lane_offset, offset, 0, 0);
+}
+
+// One fp32 through a resource: a vector-memory load for certain (a plain load of
+// an address that is the same in every lane may become a scalar one), where
+// loads in flight are counted.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t x8_rsrc_f32(const float* p, int64_t count) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, static_cast<int>(static_cast<uint32_t>(4 * count)),
+                                           kBufferWord3);
+}
+__device__ __forceinline__ float x8_load_f32(__amdgpu_buffer_rsrc_t r, uint32_t lane_offset, int offset) {
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, lane_offset, offset, 0));
+}
+
+// Four results of a row at element o (n is a multiple of 16).
+__device__ __forceinline__ void store_four(const X8Args& a, int64_t o, const f32x4& v) {
+  if (a.y_add) {  // fp32
+    float* yp = static_cast<float*>(a.y) + o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) yp[i] = add_rn(yp[i], v[i]);
+  } else if (!a.vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store_act_dt(a.y, o + i, v[i], a.y_dtype);
+  } else if (a.y_dtype == RIA_DT_F32) {
+    *reinterpret_cast<f32x4*>(static_cast<float*>(a.y) + o) = v;
+  } else {
+    const bool h = a.y_dtype == RIA_DT_F16;
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.y) + o) =
+        h ? u32x2{Kv16<RIA_DT_F16>::pack2(v[0], v[1]), Kv16<RIA_DT_F16>::pack2(v[2], v[3])}
+          : u32x2{Kv16<RIA_DT_BF16>::pack2(v[0], v[1]), Kv16<RIA_DT_BF16>::pack2(v[2], v[3])};
+  }
 }
 
 // Eight results of a row at element o.  a.vec: rows and base allow whole-vector stores.
