@@ -763,8 +763,8 @@ int ria_moe_route(int tokens, int experts, int top_k, const void* logits, int lo
  *   (g | u) = W13[e] Q(x_t),   out_t = sum_j weights[t, j] W2[e] Q(SiLU(g) u),   e = ids[t, j]
  *
  * with Q as ria_quant_fp8 and both products as ria_linear_fp8_x8.  Each slot's
- * term is rounded to out_dtype, the sum is fp32, rounded once more; with
- * accumulate, out (fp32) += it.  Slots whose id is outside [0, experts) add
+ * term is rounded to x_dtype; the sum is fp32, rounded once to out_dtype, or
+ * with accumulate added to out (fp32).  Slots whose id is outside [0, experts) add
  * nothing (a token without any gets 0); an expert may come twice in a row.
  *   x     [tokens, hidden] of x_dtype, 16-byte aligned, row stride a multiple of 8
  *   w13   [experts, 2 inter, hidden] e4m3, gate rows first; w13_scale_inv f32
@@ -795,7 +795,7 @@ typedef struct ria_moe_experts_desc {
   int64_t workspace_bytes;
 } ria_moe_experts_desc;
 
-int64_t ria_moe_experts_workspace_bytes(int tokens, int top_k, int experts, int hidden, int inter, int out_dtype);
+int64_t ria_moe_experts_workspace_bytes(int tokens, int top_k, int experts, int hidden, int inter, int x_dtype);
 int ria_moe_experts(const ria_moe_experts_desc* desc, void* stream);
 
 /*

@@ -212,6 +212,30 @@ __global__ __launch_bounds__(64 * kDealWaves) void x8_deal_kernel(const X8Args a
   }
 }
 
+// The kernel of a product.  Up to 32 rows the weights' way from HBM is all there
+// is.  Past that the kernel of the least time by rounds of its tiles over the
+// CUs, in microseconds measured on MI355X (kk = K / 2048): a round of 64 x 64
+// tiles with K dealt to four waves 1.5 + 5 kk; of 128 x 128 tiles 5 + 12 kk with
+// one a CU, 4 + 22.5 kk with two; of 256 x 256 tiles 6 + 32 kk.  Measured on
+// both sides, N = 8192, K = 2048 (64 / 128 / 256 tiles): 256 rows 15.8 / 18.0 /
+// 34.5, 512 rows 28.7 / 19.3 / 35.2, 1024 rows 53 / 29 / 37, 2048 rows 107 / 52 /
+// 42; N = 2048, K = 4096: 512 rows 12.6 / 29.8 / 61, 1536 rows 37 / 31 / 62, 8192
+// rows 193 / 99 / 77.  Wide (fp32 results), 64 / 128: 512 rows 34 / 27, and 15 / 40.
+enum class X8Plan { kFew, kDeal, kTile128, kTile256 };
+static X8Plan plan_x8(int m, int64_t t256, int64_t t128, int64_t t64, int k, bool wide) {
+  if (m <= 32) return X8Plan::kFew;
+  const int64_t cus = device_cus();
+  const double kk = k / 2048.0;
+  auto rounds = [&](int64_t tiles) { return static_cast<double>((tiles + cus - 1) / cus); };
+  const double one = wide ? 7 + 18 * kk : 5 + 12 * kk, two = wide ? 5 + 36 * kk : 4 + 22.5 * kk;
+  const int64_t rest = t128 % (2 * cus);
+  const double deal = 2 + rounds(t64) * (wide ? 1.7 + 6.2 * kk : 1.5 + 5 * kk);
+  const double tile128 = 1 + static_cast<double>(t128 / (2 * cus)) * two + (rest == 0 ? 0 : rest <= cus ? one : two);
+  const double tile256 = 2 + rounds(t256) * (6 + 32 * kk);
+  if (!wide && tile256 < tile128 && tile256 < deal) return X8Plan::kTile256;
+  return tile128 < deal ? X8Plan::kTile128 : X8Plan::kDeal;
+}
+
 bool x8_dtype_ok(int dt) { return dt == RIA_DT_BF16 || dt == RIA_DT_F16 || dt == RIA_DT_F32; }
 
 }  // namespace ria
@@ -282,27 +306,23 @@ extern "C" int ria_linear_fp8_x8(int m, int n, int k, const void* x, int64_t x_r
   if (t64 > 0x7ffffff0) return set_error(RIA_ERR_INVALID, "%s: too many rows", who);
   auto grid = [](int64_t tiles) { return dim3(static_cast<unsigned>((tiles + 7) / 8 * 8)); };
   const bool wide = y_dtype == RIA_DT_F32;
-  if (m <= 64) {
-    const int mt = m <= 16 ? 1 : m <= 32 ? 2 : 4;
+  const X8Plan plan = plan_x8(m, t256, t128, t64, k, wide);
+  if (plan == X8Plan::kFew) {
+    const bool deep = k > 4 * kFewAhead * kX8Block;  // more blocks of K than four waves hold
     const dim3 few(n / 16, 1);
-    const bool deep = k > 2048;  // blocks of K past 4 waves x kFewAhead
-    if (mt == 1 && deep)
+    if (m <= 16 && deep)
       hipLaunchKernelGGL((x8_few_kernel<1, 8>), few, dim3(512), 0, st, a);
-    else if (mt == 1)
+    else if (m <= 16)
       hipLaunchKernelGGL((x8_few_kernel<1, 4>), few, dim3(256), 0, st, a);
-    else if (mt == 2 && deep)
-      hipLaunchKernelGGL((x8_few_kernel<2, 8>), few, dim3(512), 0, st, a);
-    else if (mt == 2)
-      hipLaunchKernelGGL((x8_few_kernel<2, 4>), few, dim3(256), 0, st, a);
     else if (deep)
-      hipLaunchKernelGGL((x8_few_kernel<4, 8>), few, dim3(512), 0, st, a);
+      hipLaunchKernelGGL((x8_few_kernel<2, 8>), few, dim3(512), 0, st, a);
     else
-      hipLaunchKernelGGL((x8_few_kernel<4, 4>), few, dim3(256), 0, st, a);
-  } else if (t256 >= 192 && !wide) {
+      hipLaunchKernelGGL((x8_few_kernel<2, 4>), few, dim3(256), 0, st, a);
+  } else if (plan == X8Plan::kTile256) {
     hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 4, 2, 2, 4, false>), grid(t256), dim3(512), 0, st, a);
-  } else if (t128 >= 512 && !wide) {
+  } else if (plan == X8Plan::kTile128 && !wide) {
     hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, false>), grid(t128), dim3(256), 0, st, a);
-  } else if (t128 >= 512) {
+  } else if (plan == X8Plan::kTile128) {
     hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, true>), grid(t128), dim3(256), 0, st, a);
   } else if (!wide) {
     hipLaunchKernelGGL((x8_deal_kernel<false>), grid(t64), dim3(64 * kDealWaves), 0, st, a);

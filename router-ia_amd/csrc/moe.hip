@@ -9,6 +9,8 @@
 //     (g | u) = W13[e] Q(x_t)      Q: e4m3, a power-of-two scale per 128 values
 //     y_t     = sum_j w[t, j] W2[e_j] Q(SiLU(g) u)
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "x8_tile.h"
 
@@ -31,176 +33,281 @@ struct RouteArgs {
   int64_t w_stride;
   int32_t* ids;
   int64_t id_stride;
+  int vec;  // rows and their groups of four logits are aligned for whole loads
 };
 
-// Integers in the order of doubles: -inf lowest, NaN above every number.
-__device__ __forceinline__ int64_t order_key(double v) {
-  if (v != v) return INT64_MAX;
-  const int64_t b = __double_as_longlong(v == 0.0 ? 0.0 : v);  // -0 ranks as 0
-  return b >= 0 ? b : INT64_MIN + 1 + ~b;
+// Unsigned integers in the order of floating values: 0 for a taken or absent
+// expert, -inf above it, NaN above every number; -0 ranks as 0.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(v == 0.f ? 0.f : v);
+  return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ uint64_t order_key(double v) {
+  if (v != v) return ~uint64_t(0);
+  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v == 0.0 ? 0.0 : v));
+  return b ^ (b >> 63 ? ~uint64_t(0) : uint64_t(1) << 63);
 }
 
-__device__ __forceinline__ int64_t shfl_xor64(int64_t v, int m) {
-  const int lo = __shfl_xor(static_cast<int>(v), m), hi = __shfl_xor(static_cast<int>(v >> 32), m);
-  return (static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo);
+// The value behind an fp32 key.
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return k == 0xffffffffu ? __builtin_nanf("") : __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu));
 }
-__device__ __forceinline__ double shfl_xor_f64(double v, int m) {
-  return __longlong_as_double(shfl_xor64(__double_as_longlong(v), m));
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint64_t uniform(uint64_t v) {
+  return static_cast<uint64_t>(uniform(static_cast<uint32_t>(v >> 32))) << 32 | uniform(static_cast<uint32_t>(v));
 }
 
-// One wave per token, lane l holding experts l, l + 64, ..  Choices are compared
-// in 64 bits: a bias brings scores of unlike experts within a rounding of each
-// other, and the ids have to be the formula's.  Without a bias (and without
-// groups ranked by sums) the logits themselves are compared: scores grow with them.
-template <int XT, int V>
+// A value of lane ^ OFF, in lane exchanges of a few cycles (after the xor 8 step
+// of a reduction a rotation by 4 serves as xor 4).
+template <int OFF>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t u) {
+  if constexpr (OFF == 32 || OFF == 16) {
+    const auto r = OFF == 32 ? __builtin_amdgcn_permlane32_swap(u, u, false, false)
+                             : __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return (threadIdx.x & OFF) ? r[0] : r[1];
+  } else {
+    constexpr int kCtrl = OFF == 8 ? 0x128 : OFF == 4 ? 0x124 : OFF == 2 ? 0x4E : 0xB1;
+    return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(u), kCtrl, 0xf, 0xf, true));
+  }
+}
+template <int OFF>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t u) {
+  return static_cast<uint64_t>(lane_xor<OFF>(static_cast<uint32_t>(u >> 32))) << 32 | lane_xor<OFF>(static_cast<uint32_t>(u));
+}
+template <typename T>
+__device__ __forceinline__ T wave_max(T v) {
+  v = max(v, lane_xor<32>(v));
+  v = max(v, lane_xor<16>(v));
+  v = max(v, lane_xor<8>(v));
+  v = max(v, lane_xor<4>(v));
+  v = max(v, lane_xor<2>(v));
+  return max(v, lane_xor<1>(v));
+}
+template <>
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto r = i == 0 ? __builtin_amdgcn_permlane32_swap(v, v, false, false)
+                          : __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(r[0], r[1]);
+  }
+  v = max(v, lane_xor<8>(v));
+  v = max(v, lane_xor<4>(v));
+  v = max(v, lane_xor<2>(v));
+  return max(v, lane_xor<1>(v));
+}
+// Sum over the wave in 64 bits.
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v += __longlong_as_double(__shfl_xor(__double_as_longlong(v), m));
+  return v;
+}
+
+// exp(a - b) in fp32 from fp32 a and b: what the difference loses to rounding is
+// put back, so far-apart logits keep their relative accuracy.
+__device__ __forceinline__ float exp_diff(float a, float b) {
+  const float d = a - b;
+  const float lost = static_cast<float>((static_cast<double>(a) - static_cast<double>(b)) - static_cast<double>(d));
+  return expf(d) * (1.f + (lost == lost ? lost : 0.f));
+}
+
+// One wave per token, lane l holding experts V l .. V l + V - 1, so that of equal
+// choices the lowest lane has the lowest index.  WIDE: choices are scores in 64
+// bits (with a bias unlike scores come within an fp32 rounding of each other,
+// and the ids have to be the formula's).  Otherwise scores grow with the
+// logits, which are compared themselves.
+template <int XT, int V, bool WIDE>
 __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const RouteArgs a) {
-  __shared__ double choice_s[kRouteWaves][64 * V];
+  using Key = std::conditional_t<WIDE, uint64_t, uint32_t>;
+  __shared__ Key group_s[WIDE ? kRouteWaves : 1][WIDE ? 64 * V : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t t = (int64_t)blockIdx.x * kRouteWaves + wave;
   if (t >= a.tokens) return;
   const int e = a.experts;
-  const double ninf = -__builtin_inf();
-  double x[V], c[V];
+  const float ninf = -__builtin_inff();
+  float x[V];
+  if (V % 4 == 0 && a.vec) {  // whole groups of four, aligned
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int i = v * 64 + lane;
-    x[v] = i < e ? static_cast<double>(load_act<XT>(a.logits, t * a.stride + i)) : ninf;
-  }
-  double top = ninf, total = 0.0;
-  if (!a.sigmoid) {  // the softmax's largest logit and normaliser
+    for (int v = 0; v < V; v += 4) {
+      float f[4] = {ninf, ninf, ninf, ninf};
+      if (lane * V + v < e) load_act4<XT>(a.logits, t * a.stride + lane * V + v, f);
 #pragma unroll
-    for (int v = 0; v < V; ++v) top = x[v] > top || x[v] != x[v] ? x[v] : top;
-#pragma unroll
-    for (int m = 32; m; m >>= 1) {
-      const double o = shfl_xor_f64(top, m);
-      top = o > top || o != o ? o : top;
+      for (int i = 0; i < 4; ++i) x[(v + i) % V] = f[i];
     }
-    const double base = top == ninf ? 0.0 : top;
-    top = base;
+  } else {
 #pragma unroll
-    for (int v = 0; v < V; ++v) total += exp(x[v] - base);
+    for (int v = 0; v < V; ++v) x[v] = lane * V + v < e ? load_act<XT>(a.logits, t * a.stride + lane * V + v) : ninf;
+  }
+  // the softmax's largest logit (NaN if there is one), and in WIDE its normaliser
+  float top = 0.f;
+  double total = 1.0;
+  if (!a.sigmoid && (WIDE || !a.renorm)) {
+    uint32_t m = 0;
 #pragma unroll
-    for (int m = 32; m; m >>= 1) total += shfl_xor_f64(total, m);
+    for (int v = 0; v < V; ++v) m = max(m, order_key(x[v]));
+    m = wave_max(m);
+    top = key_value(m);
+    if (top == ninf) top = 0.f;
+    if constexpr (WIDE) {
+      double s = 0.0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) s += exp(static_cast<double>(x[v]) - static_cast<double>(top));
+      total = wave_sum64(s);
+    } else {
+      float s = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) s += exp_diff(x[v], top);
+      total = static_cast<double>(wave_sum(s));
+    }
     if (total == 0.0) total = 1.0;
   }
-  auto score = [&](double l) { return a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / total; };
-  const bool by_score = a.bias || (a.groups > 1 && a.top2);
+  Key key[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int i = v * 64 + lane;
-    c[v] = x[v];
-    if (by_score && i < e && x[v] != ninf) c[v] = score(x[v]) + (a.bias ? static_cast<double>(a.bias[i]) : 0.0);
+    const int i = lane * V + v;
+    if constexpr (WIDE) {
+      double c = x[v];
+      if (i < e && x[v] != ninf) {
+        const double l = x[v];
+        c = (a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - static_cast<double>(top)) / total) +
+            (a.bias ? static_cast<double>(a.bias[i]) : 0.0);
+      }
+      key[v] = i < e ? order_key(c) : 0;
+    } else {
+      key[v] = i < e ? order_key(x[v]) : 0;
+    }
   }
+  const Key none = WIDE ? static_cast<Key>(order_key(-__builtin_inf())) : static_cast<Key>(order_key(ninf));
   if (a.groups > 1) {
-    double* s = choice_s[wave];
-#pragma unroll
-    for (int v = 0; v < V; ++v) s[v * 64 + lane] = c[v];
-    __builtin_amdgcn_wave_barrier();
+    // rank of a group: its best key, or in WIDE with top2 the sum of its best two
     const int per = e / a.groups;
-    int64_t g = INT64_MIN;
-    if (lane < a.groups) {
-      double b0 = ninf, b1 = ninf;  // the group's best two
-      for (int i = 0; i < per; ++i) {
-        const double v = s[lane * per + i];
-        if (order_key(v) > order_key(b0)) {
-          b1 = b0;
-          b0 = v;
-        } else if (order_key(v) > order_key(b1)) {
-          b1 = v;
+    Key rank = 0;  // lane g: group g's
+    if constexpr (WIDE) {
+      Key* s = group_s[wave];
+#pragma unroll
+      for (int v = 0; v < V; ++v) s[lane * V + v] = key[v];
+      __builtin_amdgcn_wave_barrier();
+      if (lane < a.groups) {
+        Key b0 = 0, b1 = 0;
+        for (int i = 0; i < per; ++i) {
+          const Key c = s[lane * per + i];
+          b1 = max(b1, min(b0, c));
+          b0 = max(b0, c);
+        }
+        rank = b0;
+        if (a.top2 && per > 1) {
+          auto value = [](Key k) {
+            return k == ~Key(0) ? __builtin_nan("")
+                                : __longlong_as_double(static_cast<int64_t>(k ^ (k >> 63 ? Key(1) << 63 : ~Key(0))));
+          };
+          rank = order_key(value(b0) + value(b1));
         }
       }
-      g = order_key(a.top2 && per > 1 ? b0 + b1 : b0);
+    } else {
+      for (int g = 0; g < a.groups; ++g) {
+        Key m = 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int i = lane * V + v;
+          m = max(m, i >= g * per && i < (g + 1) * per ? key[v] : 0);
+        }
+        m = wave_max(m);
+        if (lane == g) rank = m;
+      }
     }
     int better = 0;  // groups that come before this one
     for (int j = 0; j < a.groups; ++j) {
-      const int lo = __shfl(static_cast<int>(g), j), hi = __shfl(static_cast<int>(g >> 32), j);
-      const int64_t o = (static_cast<int64_t>(hi) << 32) | static_cast<uint32_t>(lo);
-      better += o > g || (o == g && j < lane);
+      Key o;
+      if constexpr (WIDE)
+        o = static_cast<Key>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank >> 32), j))) << 32 |
+            static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank), j));
+      else
+        o = static_cast<Key>(__builtin_amdgcn_readlane(static_cast<int>(rank), j));
+      better += o > rank || (o == rank && j < lane);
     }
     const uint64_t open = __ballot(lane < a.groups && better < a.top_groups);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int i = v * 64 + lane;
-      if (i < e && !(open >> (i / per) & 1)) c[v] = ninf;
+      const int i = lane * V + v;
+      if (i < e && !(open >> (i / per) & 1)) key[v] = 0;
     }
   }
-  // top_k times the best that is left; ties go to the lowest index
-  int64_t key[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) key[v] = v * 64 + lane < e ? order_key(c[v]) : INT64_MIN;
-  const int64_t none = order_key(ninf);
+  // top_k times the best that is left; who holds it is scalar work, beside the other waves' vector work
   int my_id = -1;
-  double my_x = ninf;
+  float my_x = ninf;
   for (int j = 0; j < a.top_k; ++j) {
-    int64_t best = INT64_MIN;
-    int at = 0x7fffffff;
-    double bx = ninf;
+    Key head = key[0];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (key[v] > best) {  // lower indexes first
-        best = key[v];
-        at = v * 64 + lane;
-        bx = x[v];
-      }
+    for (int v = 1; v < V; ++v) head = max(head, key[v]);
+    const Key best = uniform(wave_max(head));
+    if (best <= none) break;  // the slots left over keep id -1
+    uint64_t has[V], any = 0;
 #pragma unroll
-    for (int m = 32; m; m >>= 1) {
-      const int64_t o = shfl_xor64(best, m);
-      const int oi = __shfl_xor(at, m);
-      const double ox = shfl_xor_f64(bx, m);
-      if (o > best || (o == best && oi < at)) {
-        best = o;
-        at = oi;
-        bx = ox;
-      }
+    for (int v = 0; v < V; ++v) any |= has[v] = __ballot(key[v] == best);
+    const int from = __builtin_ctzll(any);  // the lowest lane, and its first expert of that key
+    int at = V - 1;
+#pragma unroll
+    for (int v = V - 2; v >= 0; --v) at = has[v] >> from & 1 ? v : at;
+    float bx;
+    if constexpr (WIDE) {
+      bx = x[0];
+#pragma unroll
+      for (int v = 1; v < V; ++v) bx = at == v ? x[v] : bx;
+      bx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(bx), from));
+    } else {
+      bx = key_value(best);
     }
-    if (lane == j && best > none) {
-      my_id = at;
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = lane == from && at == v ? 0 : key[v];
+    if (lane == j) {
+      my_id = from * V + at;
       my_x = bx;
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (v * 64 + lane == at) key[v] = INT64_MIN;
   }
-  // weights of the chosen (lanes 0 .. top_k - 1)
-  double w = 0.0;
-  if (my_id >= 0) w = score(my_x);
+  // the chosen scores (lanes 0 .. top_k - 1)
+  float w = 0.f;
   if (a.renorm) {
-    // softmax: about the largest chosen logit, so that the weights hold where the row's largest was not chosen
-    if (!a.sigmoid) {
-      double m0 = my_x;
-#pragma unroll
-      for (int m = 32; m; m >>= 1) {
-        const double o = shfl_xor_f64(m0, m);
-        m0 = o > m0 || o != o ? o : m0;
+    // about the largest chosen logit: the weights hold where every score underflows
+    const uint32_t m = wave_max(my_id >= 0 ? order_key(my_x) : 0u);
+    const float m0 = m == 0 ? 0.f : key_value(m);
+    if (my_id >= 0) {
+      if (!a.sigmoid) {
+        w = exp_diff(my_x, m0);
+      } else {  // sigmoid(x) exp(-c), c = min(m0, 0)
+        const float c = m0 < 0.f ? m0 : 0.f;
+        w = my_x > 0.f ? 1.f / (1.f + expf(-my_x)) : exp_diff(my_x, c) / (1.f + expf(my_x));
       }
-      if (my_id >= 0) w = exp(my_x - m0) * (total != total ? total : 1.0);
     }
-    double sum = w;
-#pragma unroll
-    for (int m = 32; m; m >>= 1) sum += shfl_xor_f64(sum, m);
-    if (sum != 0.0) w /= sum;
+    if (WIDE && !a.sigmoid && total != total) w = __builtin_nanf("");  // a NaN logit that was not chosen
+    const float sum = wave_sum(w);
+    if (sum != 0.f) w = w / sum;
+  } else if (my_id >= 0) {
+    w = a.sigmoid ? 1.f / (1.f + expf(-my_x)) : static_cast<float>(static_cast<double>(exp_diff(my_x, top)) / total);
   }
   if (lane < a.top_k) {
-    a.weights[t * a.w_stride + lane] = static_cast<float>(w * static_cast<double>(a.scale));
+    a.weights[t * a.w_stride + lane] = w * a.scale;
     a.ids[t * a.id_stride + lane] = my_id;
   }
-  if (a.shared && lane == 0) {
-    const double l = static_cast<double>(load_act<XT>(a.logits, t * a.stride + e));
-    a.weights[t * a.w_stride + a.top_k] = static_cast<float>(1.0 / (1.0 + exp(-l)));
+  if (a.shared && lane == 63) {
+    const float l = load_act<XT>(a.logits, t * a.stride + e);
+    a.weights[t * a.w_stride + a.top_k] = 1.f / (1.f + expf(-l));
     a.ids[t * a.id_stride + a.top_k] = l == ninf ? -1 : e;
   }
 }
 
-template <int XT>
+template <int XT, bool WIDE>
 static void launch_route(const RouteArgs& a, hipStream_t st) {
   const dim3 grid((a.tokens + kRouteWaves - 1) / kRouteWaves), block(64 * kRouteWaves);
   const int v = (a.experts + 63) / 64;
   if (v <= 1)
-    hipLaunchKernelGGL((moe_route_kernel<XT, 1>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((moe_route_kernel<XT, 1, WIDE>), grid, block, 0, st, a);
   else if (v <= 4)
-    hipLaunchKernelGGL((moe_route_kernel<XT, 4>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((moe_route_kernel<XT, 4, WIDE>), grid, block, 0, st, a);
+  else if (v <= 8)
+    hipLaunchKernelGGL((moe_route_kernel<XT, 8, WIDE>), grid, block, 0, st, a);
   else
-    hipLaunchKernelGGL((moe_route_kernel<XT, 16>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((moe_route_kernel<XT, 16, WIDE>), grid, block, 0, st, a);
 }
 
 // ----------------------------------------------------------------------------- experts
@@ -331,27 +438,19 @@ __global__ __launch_bounds__(256) void moe_place_kernel(const PlanArgs a) {
   plan_place(a, blockIdx.x, s, e);
 }
 
-// ---- few tokens: the weights stream through registers
+// ---- a few tokens: each (token, slot) pair by itself
 //
-// A decode batch leaves an expert a handful of tokens, so the time is the
-// weights' way from HBM: each is read once, straight into MFMA operands (16
-// rows x 128 bytes of K per product, widened to fp16), by many small
-// workgroups with all of their loads in flight.  A tile is up to 16 tokens of
-// one expert, the 16 columns of a product.
-constexpr int kFewTile = 16;
+// The time is the weights' way from HBM: they go straight into MFMA operands (16
+// rows x 128 bytes of K per product, widened to fp16), by many small workgroups
+// with all of their loads in flight, and nothing is planned or sorted first.
 constexpr int kFewAhead = 4;      // blocks of K a wave loads at once
 constexpr int kFewChunk = 2048;   // hidden values quantised into LDS at a time
 
-struct FewArgs {
-  const int32_t* order;           // tiles of the plan, or (pairs mode) each pair its own tile
-  const X8Tile* tiles;
-  const int32_t* ntiles;
+struct PairsArgs {
   const int32_t* ids;
   int64_t id_stride;
-  const void* x;                  // pairs mode: x itself
+  const void* x;
   int64_t x_stride;
-  const uint8_t* x8;
-  const float* xs;
   const float* pair_w;
   int64_t pair_w_stride;
   int tokens, top_k, experts, hidden, inter;
@@ -359,226 +458,94 @@ struct FewArgs {
   const float* s13;
   const uint8_t* w2;
   const float* s2;
-  float* act;                     // [positions or pairs, inter]: SiLU(g) u
-  void* slots;
-  int slot_dtype;
-  void* out;                      // pairs mode: the sums
+  float* act;                     // [pairs, inter]: SiLU(g) u
+  void* out;
+  int out_dtype;
   int64_t out_stride;
-  int out_dtype, add;
+  int add;
 };
 
-// act = SiLU(g) u of one tile and 16 CG features, NW waves sharing K, each with
-// AH blocks of K in flight.  PAIRS: the tile is one (token, slot) pair, and x is
-// quantised here.
-template <int XT, bool PAIRS, int CG, int NW, int AH>
-__global__ __launch_bounds__(64 * NW) void moe_up_few_kernel(const FewArgs a) {
-  static_assert(64 * NW == 256 * CG, "a thread for each result of 16 rows");
-  extern __shared__ __attribute__((aligned(16))) uint8_t xq_s[];  // PAIRS: hidden e4m3 values, then their scales
-  __shared__ f32x4 red[NW][2 * CG][64];
+// act = SiLU(g) u of one pair and 16 features, four waves sharing K; x is
+// quantised here.  Column 0 of the products is the pair's (all 16 are).
+template <int XT>
+__global__ __launch_bounds__(256) void moe_up_pairs_kernel(const PairsArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t xq_s[];  // hidden e4m3 values, then their scales
+  __shared__ float red[4][2][16];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int groups = a.inter / (16 * CG);
-  const int tile = blockIdx.x / groups, c0 = blockIdx.x % groups * 16 * CG;
-  int expert, first, rows = 1;
-  if constexpr (PAIRS) {
-    first = tile;
-    expert = a.ids[(int64_t)(tile / a.top_k) * a.id_stride + tile % a.top_k];
-    if (expert < 0 || expert >= a.experts) return;
-  } else {
-    const X8Tile t = a.tiles[tile];  // in step with the count: entries past it are allocated, and not used
-    if (tile >= *a.ntiles) return;
-    expert = t.expert;
-    first = t.first;
-    rows = t.rows;
-  }
-  expert = __builtin_amdgcn_readfirstlane(expert);
+  const int groups = a.inter / 16;
+  const int pair = blockIdx.x / groups, c0 = blockIdx.x % groups * 16;
+  const int token = pair / a.top_k;
+  const int expert = __builtin_amdgcn_readfirstlane(a.ids[(int64_t)token * a.id_stride + pair % a.top_k]);
+  if (expert < 0 || expert >= a.experts) return;
   const int k = a.hidden, kblocks = k / kX8Block;
   const uint8_t* wg = a.w13 + ((int64_t)expert * 2 * a.inter + c0) * k;
   const uint8_t* wu = wg + (int64_t)a.inter * k;
   const float* sg = a.s13 + ((int64_t)expert * 2 * (a.inter / kX8Block) + c0 / kX8Block) * kblocks;
   const float* su = sg + (int64_t)(a.inter / kX8Block) * kblocks;
-  const int at = first + min(lane & 15, rows - 1);
-  const int64_t token = PAIRS ? tile / a.top_k : a.order[at] / a.top_k;
-  const uint8_t* x8 = a.x8 + token * k;
-  const float* xs = a.xs + token * kblocks;
-
-  // a wave's blocks kb0 .. kb0 + AH - 1: weights first, so that no wait for them comes early
-  u32x4 w[AH][2 * CG][2], b[AH][2];
-  float fg[AH], fu[AH], fx[AH];
-  auto load = [&](int kb0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < AH; ++i) {
-      const int kb = min(kb0 + i, kblocks - 1);
-#pragma unroll
-      for (int c = 0; c < CG; ++c) {
-        load_rows16(wg + (int64_t)16 * c * k, k, kb, lane, w[i][c]);
-        load_rows16(wu + (int64_t)16 * c * k, k, kb, lane, w[i][CG + c]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < AH; ++i) {
-      const int kb = min(kb0 + i, kblocks - 1);
-      fg[i] = sg[kb];
-      fu[i] = su[kb];
-      if constexpr (!PAIRS) {
-        load_chunks(x8 + kb * kX8Block, lane, b[i]);
-        fx[i] = xs[kb];
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);  // all of them in flight before the first product
-  };
-  load(wave * AH);
-  if constexpr (PAIRS) {
-    uint8_t* q = xq_s;
-    float* qs = reinterpret_cast<float*>(xq_s + k);
-    const int64_t x0 = token * a.x_stride;
-    for (int c = 8 * tid; c < k; c += 8 * 64 * NW) {
-      float v[8];
-      load_act8<XT>(a.x, x0 + c, v);
-      float top = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(v[i]));
-      const uint32_t e = x8_scale_exp(row16_max(top));
-      const float inv = x8_inverse(e);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = x8_value(v[i], inv);
-      *reinterpret_cast<u32x2*>(q + c) = u32x2{pack_x8(v[0], v[1], v[2], v[3]), pack_x8(v[4], v[5], v[6], v[7])};
-      if ((c & (kX8Block - 1)) == 0) qs[c / kX8Block] = x8_scale(e);
-    }
-    lds_barrier();
-  }
-  f32x4 acc[2 * CG];
-#pragma unroll
-  for (int c = 0; c < 2 * CG; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int kb0 = wave * AH; kb0 < kblocks; kb0 += NW * AH) {
-#pragma unroll
-    for (int i = 0; i < AH; ++i) {
-      const int kb = kb0 + i;
-      if (kb >= kblocks) break;
-      if constexpr (PAIRS) {
-        load_chunks(xq_s + kb * kX8Block, lane, b[i]);
-        fx[i] = reinterpret_cast<const float*>(xq_s + k)[kb];
-      }
-      const float s0 = fx[i] * fg[i], s1 = fx[i] * fu[i];
-#pragma unroll
-      for (int c = 0; c < 2 * CG; ++c) {
-        const f32x4 part = mfma_x8_16(w[i][c], b[i]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[c][j] = fmaf(part[j], c < CG ? s0 : s1, acc[c][j]);
-      }
-    }
-    if (kb0 + NW * AH < kblocks) load(kb0 + NW * AH);
-  }
-#pragma unroll
-  for (int c = 0; c < 2 * CG; ++c) red[wave][c][lane] = acc[c];
-  __syncthreads();
-  // thread (row, feature): result (feature, row) of a product is value feature % 4 of lane row + 16 (feature / 4)
-  const int row = tid / (16 * CG), f = tid % 16, c = tid / 16 % CG;
-  if (row >= rows) return;
-  float gate = 0.f, up = 0.f;
-#pragma unroll
-  for (int v = 0; v < NW; ++v) {
-    gate += red[v][c][row + 16 * (f >> 2)][f & 3];
-    up += red[v][CG + c][row + 16 * (f >> 2)][f & 3];
-  }
-  a.act[(int64_t)(first + row) * a.inter + c0 + 16 * c + f] = x8_swiglu(gate, up);
-}
-
-// 8 values of act to e4m3 at d, their block's scale to s (16 lanes a block).
-__device__ __forceinline__ void quant_act8(const float* p, uint8_t* d, float* s, int lane) {
-  const f32x4 v0 = *reinterpret_cast<const f32x4*>(p), v1 = *reinterpret_cast<const f32x4*>(p + 4);
-  float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(v[i]));
-  const uint32_t e = x8_scale_exp(row16_max(top));
-  const float inv = x8_inverse(e);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = x8_value(v[i], inv);
-  *reinterpret_cast<u32x2*>(d) = u32x2{pack_x8(v[0], v[1], v[2], v[3]), pack_x8(v[4], v[5], v[6], v[7])};
-  if ((lane & 15) == 0) *s = x8_scale(e);
-}
-
-// One tile's rows of 32 NW features of the output (a wave: 32 of them), to the
-// pairs' slots.
-template <int NW>
-__global__ __launch_bounds__(64 * NW) void moe_down_few_kernel(const FewArgs a) {
-  constexpr int kPitch = kFewChunk + 16;  // 16 rows' reads meet all banks
-  __shared__ __attribute__((aligned(16))) uint8_t h_s[kFewTile * kPitch];
-  __shared__ float hs_s[kFewTile][kFewChunk / kX8Block];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int groups = (a.hidden + 32 * NW - 1) / (32 * NW);
-  const int tile = blockIdx.x / groups;
-  const X8Tile t = a.tiles[tile];
-  if (tile >= *a.ntiles) return;
-  const int expert = __builtin_amdgcn_readfirstlane(t.expert), rows = __builtin_amdgcn_readfirstlane(t.rows);
-  const int n0 = min(blockIdx.x % groups * 32 * NW + wave * 32, a.hidden - 32);  // waves past the last feature repeat its group
-  const int k = a.inter, kblocks = k / kX8Block;
-  const uint8_t* w = a.w2 + ((int64_t)expert * a.hidden + n0) * k;
-  const float* s2 = a.s2 + ((int64_t)expert * (a.hidden / kX8Block) + n0 / kX8Block) * kblocks;
-  u32x4 v[2][kFewAhead][2];
+  u32x4 g[kFewAhead][2], u[kFewAhead][2];
+  float fg[kFewAhead], fu[kFewAhead];
   auto load = [&](int kb0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < kFewAhead; ++i) {
       const int kb = min(kb0 + i, kblocks - 1);
-      load_rows16(w, k, kb, lane, v[0][i]);
-      load_rows16(w + (int64_t)16 * k, k, kb, lane, v[1][i]);
+      load_rows16(wg, k, kb, lane, g[i]);
+      load_rows16(wu, k, kb, lane, u[i]);
     }
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int kb = min(kb0 + i, kblocks - 1);
+      fg[i] = sg[kb];
+      fu[i] = su[kb];
+    }
+    __builtin_amdgcn_sched_barrier(0);  // all of them in flight before the first product
   };
-  load(0);
-  const int row = min(lane & 15, rows - 1);
-  const int pair = a.order[t.first + row];  // ahead of the end, where its wait would show
-  const float pw = a.pair_w[(int64_t)(pair / a.top_k) * a.pair_w_stride + pair % a.top_k];
-  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-  for (int c0 = 0; c0 < k; c0 += kFewChunk) {
-    const int cols = min(kFewChunk, k - c0), units = cols / 8;
-    if (c0) __syncthreads();
-    for (int u = tid; u < rows * units; u += 64 * NW) {
-      const int r = u / units, c = (u - r * units) * 8;
-      quant_act8(a.act + (int64_t)(t.first + r) * k + c0 + c, h_s + r * kPitch + c, &hs_s[r][c / kX8Block], tid);
-    }
-    lds_barrier();
-    for (int b0 = 0; b0 < cols / kX8Block; b0 += kFewAhead) {
+  load(wave * kFewAhead);
+  float* qs = reinterpret_cast<float*>(xq_s + k);
+  for (int c = 8 * tid; c < k; c += 8 * 256) {
+    float v[8];
+    load_act8<XT>(a.x, token * a.x_stride + c, v);
+    quant_eight(v, xq_s + c, qs + c / kX8Block, tid);
+  }
+  lds_barrier();
+  f32x4 ag{0.f, 0.f, 0.f, 0.f}, au = ag;
+  for (int kb0 = wave * kFewAhead; kb0 < kblocks; kb0 += 4 * kFewAhead) {
 #pragma unroll
-      for (int i = 0; i < kFewAhead; ++i) {
-        const int kb = b0 + i;  // of the chunk
-        if (kb >= cols / kX8Block) break;
-        u32x4 b[2];
-        load_chunks(h_s + row * kPitch + kb * kX8Block, lane, b);
-        const float s = hs_s[row][kb] * s2[c0 / kX8Block + kb];
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int kb = kb0 + i;
+      if (kb >= kblocks) break;
+      u32x4 b[2];
+      load_chunks(xq_s + kb * kX8Block, lane, b);
+      const f32x4 pg = mfma_x8_16(g[i], b), pu = mfma_x8_16(u[i], b);
+      const float s0 = qs[kb] * fg[i], s1 = qs[kb] * fu[i];
 #pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          const f32x4 part = mfma_x8_16(v[f][i], b);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[f][j] = fmaf(part[j], s, acc[f][j]);
-        }
+      for (int j = 0; j < 4; ++j) {
+        ag[j] = fmaf(pg[j], s0, ag[j]);
+        au[j] = fmaf(pu[j], s1, au[j]);
       }
-      const int next = c0 / kX8Block + b0 + kFewAhead;
-      if (next < kblocks) load(next);
+    }
+    if (kb0 + 4 * kFewAhead < kblocks) load(kb0 + 4 * kFewAhead);
+  }
+  if ((lane & 15) == 0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      red[wave][0][4 * (lane >> 4) + j] = ag[j];
+      red[wave][1][4 * (lane >> 4) + j] = au[j];
     }
   }
-  if ((lane & 15) >= rows) return;
-#pragma unroll
-  for (int f = 0; f < 2; ++f) {
-    const int64_t o = (int64_t)pair * a.hidden + n0 + 16 * f + 4 * (lane >> 4);
-    float r[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = pw * acc[f][j];
-    if (a.slot_dtype == RIA_DT_F32)
-      store_act4<RIA_DT_F32>(a.slots, o, r);
-    else if (a.slot_dtype == RIA_DT_F16)
-      store_act4<RIA_DT_F16>(a.slots, o, r);
-    else
-      store_act4<RIA_DT_BF16>(a.slots, o, r);
+  __syncthreads();
+  if (tid < 16) {
+    const float gate = (red[0][0][tid] + red[1][0][tid]) + (red[2][0][tid] + red[3][0][tid]);
+    const float up = (red[0][1][tid] + red[1][1][tid]) + (red[2][1][tid] + red[3][1][tid]);
+    a.act[(int64_t)pair * a.inter + c0 + tid] = x8_swiglu(gate, up);
   }
 }
 
-// Pairs mode: 16 features of one token's sum, a wave for each slot (in turns of
+// 16 features of one token's sum, a wave for each slot (in turns of
 // kSumWaves); the terms meet in LDS and are added in slot order.
 constexpr int kSumWaves = 8;
 template <int DT>
-__global__ __launch_bounds__(64 * kSumWaves) void moe_down_pairs_kernel(const FewArgs a) {
+__global__ __launch_bounds__(64 * kSumWaves) void moe_down_pairs_kernel(const PairsArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t h_s[kSumWaves][kFewChunk];
   __shared__ float hs_s[kSumWaves][kFewChunk / kX8Block];
   __shared__ float term[kSumWaves][16];
@@ -605,8 +572,11 @@ __global__ __launch_bounds__(64 * kSumWaves) void moe_down_pairs_kernel(const Fe
 #pragma unroll
           for (int i = 0; i < kFewAhead; ++i) load_rows16(w, k, min(c0 / kX8Block + b0 + i, kblocks - 1), lane, v[i]);
           if (b0 == 0)  // 64 lanes: four blocks at a time (whole groups of 16 lanes)
-            for (int c = 8 * lane; c < cols; c += 8 * 64)
-              quant_act8(act + c0 + c, h_s[wave] + c, &hs_s[wave][c / kX8Block], lane);
+            for (int c = 8 * lane; c < cols; c += 8 * 64) {
+              float h[8];
+              load_act8<RIA_DT_F32>(act, c0 + c, h);
+              quant_eight(h, h_s[wave] + c, &hs_s[wave][c / kX8Block], lane);
+            }
           __builtin_amdgcn_wave_barrier();
 #pragma unroll
           for (int i = 0; i < kFewAhead; ++i) {
@@ -635,19 +605,18 @@ __global__ __launch_bounds__(64 * kSumWaves) void moe_down_pairs_kernel(const Fe
   }
   if (tid < 16) {
     const int64_t o = (int64_t)t * a.out_stride + n0 + tid;
-    if constexpr (DT == RIA_DT_F32) {
-      if (a.add) sum = add_rn(static_cast<const float*>(a.out)[o], sum);
-    }
-    store_act<DT>(a.out, o, sum);
+    if (a.add) sum = add_rn(static_cast<const float*>(a.out)[o], sum);
+    store_act_dt(a.out, o, sum, a.out_dtype);
   }
 }
 
 struct CombineArgs {
-  const void* slots;  // [tokens * top_k, hidden], in out's dtype
+  const void* slots;  // [tokens * top_k, hidden], in x's dtype
   const int32_t* ids;
   int64_t id_stride;
   int tokens, top_k, experts, hidden;
   void* out;
+  int out_dtype;
   int64_t out_stride;
   int add, vec;
 };
@@ -681,7 +650,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs a) {
   }
   X8Args o{};
   o.y = a.out;
-  o.y_dtype = DT;
+  o.y_dtype = a.out_dtype;
   o.y_add = a.add;
   o.vec = a.vec;
   store_eight(o, t * a.out_stride + c, s);
@@ -694,24 +663,31 @@ static int64_t moe_tiles(int64_t pairs, int experts, int tile) {
   return std::min<int64_t>(pairs, pairs / tile + std::min<int64_t>(experts, pairs));
 }
 
-// How a call is run, by its pairs: each pair by itself, tiles of 16 pairs whose
-// weights stream through registers, or tiles of 64 or 256 pairs in LDS.
-enum class MoeKind { kPairs, kFew, kTiles };
-static MoeKind moe_kind(int64_t pairs, int experts) {
-  if (pairs <= 32) return MoeKind::kPairs;
-  return pairs <= (int64_t)experts * 8 ? MoeKind::kFew : MoeKind::kTiles;
+// Whether each pair is run by itself.  That reads an expert's weights again for
+// each further pair of it, but saves the planning and combining launches, some
+// 10 us: with the pairs spread evenly, up to 40 MB of repeated weights.
+// Measured by pairs / in tiles of 64 (experts, top_k, hidden, inter): (256, 8,
+// 2048, 512) 8 tokens 39 / 49 us, 16 tokens 67 / 75, 32 tokens 118 / 113; (16, 2,
+// 2048, 1024) 8 tokens 25 / 33, 16 tokens 38 / 34; (60, 4, 1024, 768) 8 tokens
+// 24 / 27, 16 tokens 40 / 30.
+static bool moe_by_pairs(int64_t pairs, int experts, int hidden, int inter) {
+  if (pairs > 512) return false;
+  const double met = experts * (1.0 - std::pow(1.0 - 1.0 / experts, static_cast<double>(pairs)));
+  return (pairs - met) * 3.0 * hidden * inter <= 40e6;
 }
 
-// Pairs of one expert that a tile takes.
-static int moe_tile(int64_t pairs, int experts, int out_dtype) {
-  if (moe_kind(pairs, experts) != MoeKind::kTiles) return kFewTile;
-  return out_dtype != RIA_DT_F32 && pairs >= (int64_t)experts * 128 ? 256 : 64;
+// Pairs of one expert that a tile takes.  256 from 192 pairs an expert on,
+// where full tiles outweigh what the last ones leave empty: (256, 8, 2048, 512)
+// 2048 tokens 243 us in tiles of 64, 300 of 256, 4096 tokens 338 and 357, 8192
+// tokens 564 and 533.  (fp32 x has no kernel of 256.)
+static int moe_tile(int64_t pairs, int experts, int x_dtype) {
+  return x_dtype != RIA_DT_F32 && pairs >= (int64_t)experts * 192 ? 256 : 64;
 }
 
 struct MoeLayout {
   int64_t x8, xs, counts, order, tiles, ntiles, act, h8, hs, slots, bytes;
 };
-static MoeLayout moe_layout(int64_t tokens, int top_k, int experts, int hidden, int inter, int out_dtype) {
+static MoeLayout moe_layout(int64_t tokens, int top_k, int experts, int hidden, int inter, int x_dtype) {
   MoeLayout l{};
   const int64_t pairs = tokens * top_k;
   int64_t at = 0;
@@ -720,17 +696,19 @@ static MoeLayout moe_layout(int64_t tokens, int top_k, int experts, int hidden, 
     at += align256(bytes);
     return here;
   };
-  l.x8 = take(tokens * hidden);
-  l.xs = take(tokens * (hidden / kX8Block) * 4);
-  l.counts = take((pairs + kPlanPairs - 1) / kPlanPairs * experts * 4);
-  l.order = take(pairs * 4);
-  l.tiles = take(moe_tiles(pairs, experts, moe_tile(pairs, experts, out_dtype)) * static_cast<int64_t>(sizeof(X8Tile)));
-  l.ntiles = take(4);
-  const bool tiled = moe_kind(pairs, experts) == MoeKind::kTiles;
-  l.act = take(tiled ? 0 : pairs * inter * 4);
-  l.h8 = take(tiled ? pairs * inter : 0);
-  l.hs = take(tiled ? pairs * (inter / kX8Block) * 4 : 0);
-  l.slots = take(pairs * hidden * (out_dtype == RIA_DT_F32 ? 4 : 2));
+  if (moe_by_pairs(pairs, experts, hidden, inter)) {
+    l.act = take(pairs * inter * 4);
+  } else {
+    l.x8 = take(tokens * hidden);
+    l.xs = take(tokens * (hidden / kX8Block) * 4);
+    l.counts = take((pairs + kPlanPairs - 1) / kPlanPairs * experts * 4);
+    l.order = take(pairs * 4);
+    l.tiles = take(moe_tiles(pairs, experts, moe_tile(pairs, experts, x_dtype)) * static_cast<int64_t>(sizeof(X8Tile)));
+    l.ntiles = take(4);
+    l.h8 = take(pairs * inter);
+    l.hs = take(pairs * (inter / kX8Block) * 4);
+    l.slots = take(pairs * hidden * (x_dtype == RIA_DT_F32 ? 4 : 2));
+  }
   l.bytes = at;
   return l;
 }
@@ -755,12 +733,18 @@ static void launch_moe_tiles(const ria_moe_experts_desc& d, const MoeLayout& l, 
   up.h8 = static_cast<uint8_t*>(at(l.h8));
   up.hs = static_cast<float*>(at(l.hs));
   up.m = d.tokens;
-  const bool wide = d.out_dtype == RIA_DT_F32;
+  const bool wide = d.x_dtype == RIA_DT_F32;
+  // most experts' pairs fill one tile: their weights are read once, and kept in no cache
+  const bool once = (int64_t)d.tokens * d.top_k <= (int64_t)d.experts * 32;
   auto grid_of = [&](int feature_tiles) { return dim3(static_cast<unsigned>((most * feature_tiles + 7) / 8 * 8)); };
-  if (wide)
+  if (wide && once)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
+  else if (wide)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   else if (tile == 256)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 4, 2, 2, 4, false>), grid_of(d.inter / 128), dim3(512), 0, st, up);
+  else if (once)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   else
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   X8Args dn = up;
@@ -774,14 +758,18 @@ static void launch_moe_tiles(const ria_moe_experts_desc& d, const MoeLayout& l, 
   dn.k = d.inter;
   dn.y = at(l.slots);
   dn.y_stride = d.hidden;
-  dn.y_dtype = d.out_dtype;
+  dn.y_dtype = d.x_dtype;
   dn.vec = 1;
   dn.pair_w = d.weights;
   dn.pair_w_stride = d.weights_row_stride;
-  if (wide)
+  if (wide && once)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, true, true>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
+  else if (wide)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, true>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
   else if (tile == 256)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 4, 2, 2, 4, false>), grid_of((d.hidden + 255) / 256), dim3(512), 0, st, dn);
+  else if (once)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, false, true>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
   else
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, false>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
 }
@@ -821,23 +809,34 @@ extern "C" int ria_moe_route(int tokens, int experts, int top_k, const void* log
   const int s = shared_expert ? 1 : 0;
   if (logits_row_stride < experts + s || weights_row_stride < top_k + s || ids_row_stride < top_k + s)
     return set_error(RIA_ERR_INVALID, "%s: row stride too small", who);
+  const int size = logits_dtype == RIA_DT_F32 ? 4 : 2;
+  const bool vec = experts % 4 == 0 && logits_row_stride % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % (4 * size) == 0;
   const RouteArgs a{logits, logits_row_stride, tokens, experts, top_k, bias, scoring == RIA_ROUTE_SIGMOID, num_groups,
                     top_groups, group_score == RIA_ROUTE_GROUP_TOP2, renormalize != 0, s, scale, weights,
-                    weights_row_stride, ids, ids_row_stride};
+                    weights_row_stride, ids, ids_row_stride, vec};
+  // scores need comparing where a bias or a sum of two stands between them and the logits
+  const bool wide = bias || (num_groups > 1 && group_score == RIA_ROUTE_GROUP_TOP2);
   hipStream_t st = static_cast<hipStream_t>(stream);
+  auto launch = [&](auto dt) {
+    constexpr int XT = decltype(dt)::value;
+    if (wide)
+      launch_route<XT, true>(a, st);
+    else
+      launch_route<XT, false>(a, st);
+  };
   if (logits_dtype == RIA_DT_BF16)
-    launch_route<RIA_DT_BF16>(a, st);
+    launch(std::integral_constant<int, RIA_DT_BF16>{});
   else if (logits_dtype == RIA_DT_F16)
-    launch_route<RIA_DT_F16>(a, st);
+    launch(std::integral_constant<int, RIA_DT_F16>{});
   else
-    launch_route<RIA_DT_F32>(a, st);
+    launch(std::integral_constant<int, RIA_DT_F32>{});
   return check_launch(who);
 }
 
 extern "C" int64_t ria_moe_experts_workspace_bytes(int tokens, int top_k, int experts, int hidden, int inter,
-                                                   int out_dtype) {
-  if (moe_sizes_error(tokens, top_k, experts, hidden, inter) || !x8_dtype_ok(out_dtype)) return -1;
-  return moe_layout(tokens, top_k, experts, hidden, inter, out_dtype).bytes;
+                                                   int x_dtype) {
+  if (moe_sizes_error(tokens, top_k, experts, hidden, inter) || !x8_dtype_ok(x_dtype)) return -1;
+  return moe_layout(tokens, top_k, experts, hidden, inter, x_dtype).bytes;
 }
 
 extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
@@ -857,49 +856,44 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
   if ((reinterpret_cast<uintptr_t>(d->w13) | reinterpret_cast<uintptr_t>(d->w2)) % 16)
     return set_error(RIA_ERR_INVALID, "%s: the weights must be 16-byte aligned", who);
   if (reinterpret_cast<uintptr_t>(d->workspace) % 256) return set_error(RIA_ERR_INVALID, "%s: workspace must be 256-byte aligned", who);
-  const MoeLayout l = moe_layout(d->tokens, d->top_k, d->experts, d->hidden, d->inter, d->out_dtype);
+  const MoeLayout l = moe_layout(d->tokens, d->top_k, d->experts, d->hidden, d->inter, d->x_dtype);
   if (d->workspace_bytes < l.bytes)
     return set_error(RIA_ERR_WORKSPACE, "%s: workspace of %lld bytes, %lld needed", who, (long long)d->workspace_bytes,
                      (long long)l.bytes);
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(d->workspace);
   auto at = [&](int64_t o) { return static_cast<void*>(ws + o); };
-  int32_t* order = static_cast<int32_t*>(at(l.order));
-  X8Tile* tiles = static_cast<X8Tile*>(at(l.tiles));
-  int32_t* ntiles = static_cast<int32_t*>(at(l.ntiles));
   const int64_t pairs = (int64_t)d->tokens * d->top_k;
-  const MoeKind kind = moe_kind(pairs, d->experts);
-  const int tile = moe_tile(pairs, d->experts, d->out_dtype);
-  const int64_t most = moe_tiles(pairs, d->experts, tile);
-  if (std::max(most, pairs) * (std::max(d->hidden, d->inter) / 16) > 0x7ffffff0)
-    return set_error(RIA_ERR_INVALID, "%s: too many (token, slot) pairs", who);
-  FewArgs few{order, tiles, ntiles, d->ids, d->ids_row_stride, d->x, d->x_row_stride,
-              static_cast<const uint8_t*>(at(l.x8)), static_cast<const float*>(at(l.xs)), d->weights,
-              d->weights_row_stride, d->tokens, d->top_k, d->experts, d->hidden, d->inter,
-              static_cast<const uint8_t*>(d->w13), d->w13_scale_inv, static_cast<const uint8_t*>(d->w2),
-              d->w2_scale_inv, static_cast<float*>(at(l.act)), at(l.slots), d->out_dtype, d->out, d->out_row_stride,
-              d->out_dtype, d->accumulate != 0};
-  if (kind == MoeKind::kPairs) {
+  if (moe_by_pairs(pairs, d->experts, d->hidden, d->inter)) {
+    const PairsArgs p{d->ids, d->ids_row_stride, d->x, d->x_row_stride, d->weights, d->weights_row_stride, d->tokens,
+                      d->top_k, d->experts, d->hidden, d->inter, static_cast<const uint8_t*>(d->w13), d->w13_scale_inv,
+                      static_cast<const uint8_t*>(d->w2), d->w2_scale_inv, static_cast<float*>(at(l.act)), d->out,
+                      d->out_dtype, d->out_row_stride, d->accumulate != 0};
     const dim3 ugrid(static_cast<unsigned>(pairs * (d->inter / 16)));
     const dim3 dgrid(static_cast<unsigned>((int64_t)d->tokens * (d->hidden / 16)));
     const size_t lds = d->hidden + d->hidden / kX8Block * 4;
     if (d->x_dtype == RIA_DT_BF16)
-      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_BF16, true, 1, 4, 4>), ugrid, dim3(256), lds, st, few);
+      hipLaunchKernelGGL((moe_up_pairs_kernel<RIA_DT_BF16>), ugrid, dim3(256), lds, st, p);
     else if (d->x_dtype == RIA_DT_F16)
-      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F16, true, 1, 4, 4>), ugrid, dim3(256), lds, st, few);
+      hipLaunchKernelGGL((moe_up_pairs_kernel<RIA_DT_F16>), ugrid, dim3(256), lds, st, p);
     else
-      hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F32, true, 1, 4, 4>), ugrid, dim3(256), lds, st, few);
-    if (d->out_dtype == RIA_DT_BF16)
-      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_BF16>), dgrid, dim3(64 * kSumWaves), 0, st, few);
-    else if (d->out_dtype == RIA_DT_F16)
-      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_F16>), dgrid, dim3(64 * kSumWaves), 0, st, few);
+      hipLaunchKernelGGL((moe_up_pairs_kernel<RIA_DT_F32>), ugrid, dim3(256), lds, st, p);
+    if (d->x_dtype == RIA_DT_BF16)
+      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_BF16>), dgrid, dim3(64 * kSumWaves), 0, st, p);
+    else if (d->x_dtype == RIA_DT_F16)
+      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_F16>), dgrid, dim3(64 * kSumWaves), 0, st, p);
     else
-      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_F32>), dgrid, dim3(64 * kSumWaves), 0, st, few);
+      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_F32>), dgrid, dim3(64 * kSumWaves), 0, st, p);
     return check_launch(who);
   }
+  const int tile = moe_tile(pairs, d->experts, d->x_dtype);
+  const int64_t most = moe_tiles(pairs, d->experts, tile);
+  if (most * (std::max(d->hidden, d->inter) / 128) > 0x7ffffff0)
+    return set_error(RIA_ERR_INVALID, "%s: too many (token, slot) pairs", who);
   const PlanArgs plan{d->ids, d->ids_row_stride, static_cast<int>(pairs), d->top_k, d->experts,
                       static_cast<int>((pairs + kPlanPairs - 1) / kPlanPairs), tile, static_cast<int32_t*>(at(l.counts)),
-                      order, tiles, ntiles};
+                      static_cast<int32_t*>(at(l.order)), static_cast<X8Tile*>(at(l.tiles)),
+                      static_cast<int32_t*>(at(l.ntiles))};
   const QuantArgs quant{d->tokens * (int64_t)(d->hidden / 8), d->hidden / 8, d->x, d->x_row_stride,
                         static_cast<uint8_t*>(at(l.x8)), static_cast<float*>(at(l.xs))};
   const dim3 pgrid(static_cast<unsigned>(plan.blocks + (quant.units + 255) / 256));
@@ -910,20 +904,14 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
   else
     hipLaunchKernelGGL((moe_prepare_kernel<RIA_DT_F32>), pgrid, dim3(256), 0, st, plan, quant);
   if (plan.blocks > 1) hipLaunchKernelGGL(moe_place_kernel, dim3(plan.blocks), dim3(256), 0, st, plan);
-  if (kind == MoeKind::kFew) {
-    hipLaunchKernelGGL((moe_up_few_kernel<RIA_DT_F32, false, 2, 8, 2>), dim3(static_cast<unsigned>(most * (d->inter / 32))),
-                       dim3(512), 0, st, few);
-    hipLaunchKernelGGL((moe_down_few_kernel<4>), dim3(static_cast<unsigned>(most * (d->hidden / 128))), dim3(256), 0, st, few);
-  } else {
-    launch_moe_tiles(*d, l, most, tile, st);
-  }
+  launch_moe_tiles(*d, l, most, tile, st);
   const CombineArgs c{at(l.slots), d->ids, d->ids_row_stride, d->tokens, d->top_k, d->experts, d->hidden, d->out,
-                      d->out_row_stride, d->accumulate != 0,
+                      d->out_dtype, d->out_row_stride, d->accumulate != 0,
                       reinterpret_cast<uintptr_t>(d->out) % 16 == 0 && d->out_row_stride % 8 == 0};
   const dim3 grid(static_cast<unsigned>(((int64_t)d->tokens * (d->hidden / 8) + 255) / 256));
-  if (d->out_dtype == RIA_DT_BF16)
+  if (d->x_dtype == RIA_DT_BF16)
     hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_BF16>), grid, dim3(256), 0, st, c);
-  else if (d->out_dtype == RIA_DT_F16)
+  else if (d->x_dtype == RIA_DT_F16)
     hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F16>), grid, dim3(256), 0, st, c);
   else
     hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F32>), grid, dim3(256), 0, st, c);

@@ -127,6 +127,19 @@ __device__ __forceinline__ float x8_swiglu(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
 }
 
+// Eight values of a block to e4m3 at d; the first of its 16 lanes stores the scale.
+__device__ __forceinline__ void quant_eight(float (&v)[8], uint8_t* d, float* s, int lane) {
+  float top = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(v[i]));
+  const uint32_t e = x8_scale_exp(row16_max(top));
+  const float inv = x8_inverse(e);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = x8_value(v[i], inv);
+  *reinterpret_cast<u32x2*>(d) = u32x2{pack_x8(v[0], v[1], v[2], v[3]), pack_x8(v[4], v[5], v[6], v[7])};
+  if ((lane & 15) == 0) *s = x8_scale(e);
+}
+
 struct QuantArgs {
   int64_t units;     // rows * per_row
   int per_row;       // 8 values each
@@ -144,15 +157,7 @@ __device__ __forceinline__ void quant_unit(const QuantArgs& a, int64_t u) {
   const int c = static_cast<int>(u - r * a.per_row) * 8;
   float v[8];
   load_act8<XT>(a.x, r * a.x_stride + c, v);
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(v[i]));
-  const uint32_t e = x8_scale_exp(row16_max(top));
-  const float inv = x8_inverse(e);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = x8_value(v[i], inv);
-  *reinterpret_cast<u32x2*>(a.out + u * 8) = u32x2{pack_x8(v[0], v[1], v[2], v[3]), pack_x8(v[4], v[5], v[6], v[7])};
-  if ((u & 15) == 0) a.scale[u / 16] = x8_scale(e);
+  quant_eight(v, a.out + u * 8, a.scale + u / 16, static_cast<int>(u & 15));
 }
 
 // ---- the tiled product
@@ -196,8 +201,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t x8_rsrc(const uint8_t* p, int6
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, static_cast<int>(static_cast<uint32_t>(bytes)),
                                            kBufferWord3);
 }
+template <bool STREAM = false>  // read once: not kept in the caches
 __device__ __forceinline__ void x8_copy(__amdgpu_buffer_rsrc_t r, uint8_t* d, uint32_t lane_offset, int offset) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, d, 16, lane_offset, offset, 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, d, 16, lane_offset, offset, 0, STREAM ? 2 : 0);
 }
 
 // One fp32 through a resource: a vector-memory load for certain (a plain load of
@@ -276,7 +282,7 @@ __device__ __forceinline__ int x8_order(int b, int total) {
 // step stages one block of K, 128 bytes a row, in LDS by direct copies, chunk
 // c of row r at chunk c ^ ((r >> 1) & 7), so that the 16 lanes of a read's
 // phase meet all 64 banks; the next step's copies run beside the products.
-template <int MODE, int WF, int WT, int NF, int NT, bool WIDE>
+template <int MODE, int WF, int WT, int NF, int NT, bool WIDE, bool STREAM = false>
 __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
   constexpr int NW = NF * NT;
   constexpr int BN = 32 * WF * NF, BM = 32 * WT * NT;
@@ -357,7 +363,7 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
   auto issue = [&](int kb) __attribute__((always_inline)) {
     uint8_t* d = lds + (kb & 1) * kStep;
 #pragma unroll
-    for (int i = 0; i < WL; ++i) x8_copy(wr, d + (wave * WL + i) * 1024, wo[i], kb * kX8Block);
+    for (int i = 0; i < WL; ++i) x8_copy<STREAM>(wr, d + (wave * WL + i) * 1024, wo[i], kb * kX8Block);
 #pragma unroll
     for (int i = 0; i < XL; ++i) x8_copy(xr, d + BN * kX8Block + (wave * XL + i) * 1024, xo[i], kb * kX8Block);
   };

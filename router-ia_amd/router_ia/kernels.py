@@ -1300,9 +1300,9 @@ def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bia
 
 
 def moe_experts_workspace_bytes(tokens: int, top_k: int, experts: int, hidden: int, inter: int,
-                                out_dtype: torch.dtype = torch.float16) -> int:
+                                x_dtype: torch.dtype = torch.float16) -> int:
     """Bytes of the workspace moe_experts takes for these sizes (ria_moe_experts_workspace_bytes)."""
-    n = nat.load().ria_moe_experts_workspace_bytes(tokens, top_k, experts, hidden, inter, _DTYPE_CODE[out_dtype])
+    n = nat.load().ria_moe_experts_workspace_bytes(tokens, top_k, experts, hidden, inter, _DTYPE_CODE[x_dtype])
     if n < 0:
         raise ValueError(f"sizes refused: {tokens} tokens x {top_k} of {experts} experts, hidden {hidden}, inter {inter}")
     return n
@@ -1328,7 +1328,8 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: 
     int32 and weights fp32 [T, k] as moe_route gives them (ids outside the
     experts add nothing); w13 [E, 2 I, H] (gate rows first) and w2 [E, H, I]
     float8_e4m3fn with fp32 scales per 128x128 block, H and I multiples of
-    128.  Returns / fills out [T, H] (x's dtype unless out_dtype or out says
+    128.  Each slot's term is rounded to x's dtype, their fp32 sum once to
+    out's.  Returns / fills out [T, H] (x's dtype unless out_dtype or out says
     otherwise); with ``accumulate`` the fp32 ``out`` receives out + the sum.
     ``workspace``: uint8, moe_experts_workspace_bytes (allocated if not given);
     calls that may overlap need one each.
@@ -1361,7 +1362,7 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: 
         if accumulate and out.dtype != torch.float32:
             raise ValueError("accumulate needs an fp32 out")
     if workspace is None:
-        workspace = torch.empty(moe_experts_workspace_bytes(t, k, e, h, i, out.dtype), dtype=torch.uint8,
+        workspace = torch.empty(moe_experts_workspace_bytes(t, k, e, h, i, x.dtype), dtype=torch.uint8,
                                 device=x.device)
     else:
         _require_gpu("workspace", workspace, x.device)

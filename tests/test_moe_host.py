@@ -128,7 +128,7 @@ def test_experts_refusals() -> None:
 def test_workspace_sizes() -> None:
     small, large = (K.moe_experts_workspace_bytes(t, 8, 256, 2048, 512) for t in (1, 4096))
     assert 0 < small < large
-    assert K.moe_experts_workspace_bytes(1, 8, 256, 2048, 512, torch.float32) > small
+    assert K.moe_experts_workspace_bytes(4096, 8, 256, 2048, 512, torch.float32) > large
     with pytest.raises(ValueError, match="sizes refused"):
         K.moe_experts_workspace_bytes(1, 8, 256, 2000, 512)
 
