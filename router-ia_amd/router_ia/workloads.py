@@ -161,3 +161,21 @@ def synthetic_layer(seed: int, model_layer: int, device="cpu", on_device: bool =
         out["linear_attn.dt_bias"] = p["dt_bias"]
         out["linear_attn.norm.weight"] = norms["gated_norm"]
     return out
+
+
+def synthetic_moe_layer(seed: int, experts: int, inter: int, hidden: int = 2048, shared: bool = True,
+                        device="cpu", on_device: bool = False) -> dict[str, torch.Tensor]:
+    """One layer's mixture-of-experts weights as a checkpoint holds them, keyed by the checkpoint's suffixes."""
+    g = _gen(seed, "cpu")
+    out = {"post_attention_layernorm.weight": (torch.randn((hidden,), generator=g) * 0.1).to(torch.bfloat16).to(device),
+           "mlp.gate.weight": (torch.randn((experts, hidden), generator=g) * 0.02).to(torch.bfloat16).to(device)}
+    names = [f"mlp.experts.{e}." for e in range(experts)]
+    if shared:
+        out["mlp.shared_expert_gate.weight"] = (torch.randn((1, hidden), generator=g) * 0.02).to(torch.bfloat16).to(device)
+        names.append("mlp.shared_expert.")
+    for j, name in enumerate(names):
+        for i, (proj, n, k) in enumerate((("gate_proj", inter, hidden), ("up_proj", inter, hidden),
+                                          ("down_proj", hidden, inter))):
+            w8, s = fp8_block_weight(seed * 4096 + 3 * j + i, n, k, 0.02, device=device, on_device=on_device)
+            out[f"{name}{proj}.weight"], out[f"{name}{proj}.weight_scale_inv"] = w8, s
+    return out

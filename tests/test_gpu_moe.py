@@ -152,7 +152,7 @@ def test_quant_edges(gpu):
 LINEAR = [  # (m, n, k)
     (1, 16, 128), (1, 8192, 2048), (2, 48, 256), (5, 400, 1152), (16, 512, 2048), (17, 2048, 4096), (33, 144, 128),
     (64, 1040, 640), (100, 2048, 512), (129, 272, 2048), (200, 1536, 384), (300, 2048, 4096), (513, 784, 896),
-    (1025, 4112, 256),
+    (1025, 4112, 256), (40, 96, 128), (70, 80, 384), (4001, 4080, 384),
 ]
 
 
@@ -305,7 +305,7 @@ def test_route_extreme_logits(gpu):
 EXPERTS = [  # (tokens, experts, top_k, hidden, inter)
     (1, 8, 2, 256, 128), (1, 16, 8, 2048, 512), (2, 4, 1, 128, 128), (3, 5, 5, 384, 256), (7, 16, 3, 512, 640),
     (17, 3, 2, 256, 128), (40, 33, 4, 256, 384), (130, 6, 2, 640, 256), (200, 2, 2, 256, 128), (300, 40, 6, 512, 128),
-    (700, 3, 2, 256, 256),
+    (700, 3, 2, 256, 256), (2100, 5, 2, 256, 128),
 ]
 
 
@@ -354,3 +354,191 @@ def test_experts_match_definition(gpu, t, e, k, h, i, dtype):
     tight = expert_tolerance(want, mag, k, dtype, 0.0)
     moved = int((err > tight).any(-1).sum())
     assert moved <= 1 + math.ceil(t * k * i * 2.0 ** -17), f"{moved} of {t} rows"
+
+
+def device(a, gpu):
+    return [v.to(gpu) for v in a]
+
+
+def check_experts(out, want, mag, k, i, dtype):
+    err = (out.cpu().double() - want).abs()
+    tol = expert_tolerance(want, mag, k, dtype, 0.125 * 4 * 2 / math.sqrt(i))
+    assert bool((err <= tol).all()), f"{(err / tol).max().item():.3g} of the tolerance"
+
+
+@pytest.mark.parametrize("t", [1, 9, 150])
+def test_experts_accumulate_strided_and_on_another_stream(gpu, t):
+    """16-bit x into an fp32 residual stream: rows of wider buffers, a workspace of the caller's, another stream."""
+    announce(f"moe_experts: {t} tokens, accumulate")
+    e, k, h, i = 6, 2, 384, 256
+    x, ids, weights, *w = expert_inputs(t, e, k, h, i, torch.float16, 77 + t)
+    want, mag = experts64(x, ids, weights, *w)
+    base = torch.randn((t, h + 12), generator=gen(5))
+    out = base.to(gpu)
+    wide_x = torch.nn.functional.pad(x, (0, 8)).to(gpu)[:, :h]
+    wide_ids = torch.nn.functional.pad(ids, (0, 3)).to(gpu)[:, :k]
+    wide_w = torch.nn.functional.pad(weights, (0, 5)).to(gpu)[:, :k]
+    w = device(w, gpu)
+    ws = torch.empty(K.moe_experts_workspace_bytes(t, k, e, h, i) + 7, dtype=torch.uint8, device=gpu)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = K.moe_experts(wide_x, wide_ids, wide_w, *w, out=out[:, 4:4 + h], accumulate=True, workspace=ws)
+    side.synchronize()
+    assert got.data_ptr() == out[:, 4:].data_ptr()
+    out = out.cpu()
+    assert torch.equal(out[:, :4], base[:, :4]) and torch.equal(out[:, 4 + h:], base[:, 4 + h:])
+    # the terms are fp16 (x's type), their sum and the residual fp32
+    err = (out[:, 4:4 + h].double() - base[:, 4:4 + h].double() - want).abs()
+    tol = expert_tolerance(want, mag, k, torch.float16, 0.125 * 4 * 2 / math.sqrt(i)) + 2.0 ** -23 * out[:, 4:4 + h].abs()
+    assert bool((err <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("t", [2, 70, 1200])
+def test_experts_all_tokens_to_one_expert_and_twice(gpu, t, dtype):
+    """The whole batch on one expert (the others' tiles empty), some rows naming it in both slots."""
+    announce(f"moe_experts: {t} tokens on one expert of 7")
+    e, k, h, i = 7, 2, 256, 128
+    x, ids, weights, *w = expert_inputs(t, e, k, h, i, dtype, 3)
+    ids[:] = 5
+    ids[1::2, 1] = -7
+    want, mag = experts64(x, ids, weights, *w)
+    out = K.moe_experts(*device((x, ids, weights, *w), gpu))
+    check_experts(out, want, mag, k, i, dtype)
+
+
+@pytest.mark.parametrize("t", [3, 90])
+def test_experts_without_any(gpu, t):
+    """No slot names an expert: zeros, also over what out held; with accumulate out stays."""
+    announce("moe_experts: every id out of range")
+    e, k, h, i = 4, 3, 256, 128
+    x, ids, weights, *w = device(expert_inputs(t, e, k, h, i, torch.bfloat16, 9), gpu)
+    ids.fill_(-1)
+    ids[:, 1] = e
+    ids[:, 2] = 2 ** 31 - 1
+    out = torch.full((t, h), math.nan, dtype=torch.bfloat16, device=gpu)
+    K.moe_experts(x, ids, weights, *w, out=out)
+    assert not bool(out.any())
+    keep = torch.randn((t, h), device=gpu)
+    out = keep.clone()
+    K.moe_experts(x, ids, weights, *w, out=out, accumulate=True)
+    assert torch.equal(out, keep)
+
+
+@pytest.mark.parametrize("t", [4, 100])
+def test_experts_nan_and_infinity_stay_in_their_token(gpu, t):
+    announce("moe_experts: NaN and infinite activations")
+    e, k, h, i = 5, 2, 256, 128
+    x, ids, weights, *w = expert_inputs(t, e, k, h, i, torch.float16, 21)
+    x[1, 7], x[3, 200] = math.nan, math.inf
+    out = K.moe_experts(*device((x, ids, weights, *w), gpu)).cpu()
+    bad = torch.isnan(out)
+    assert bool(bad[1].all()) and bool(bad[3].all())
+    rest = torch.tensor([r for r in range(t) if r not in (1, 3)])
+    assert not bool(bad[rest].any())
+    want, mag = experts64(x[rest], ids[rest], weights[rest], *w)
+    check_experts(out[rest], want, mag, k, i, torch.float16)
+
+
+def test_experts_same_inputs_same_bits(gpu):
+    """Which place a pair gets in its expert's tiles is left to the order of the counting: the results are not."""
+    announce("moe_experts: repeated calls")
+    for t, e, k in ((8, 16, 4), (900, 6, 2), (3000, 6, 2)):
+        a = device(expert_inputs(t, e, k, 256, 256, torch.bfloat16, t), gpu)
+        first = K.moe_experts(*a)
+        for _ in range(4):
+            assert torch.equal(K.moe_experts(*a), first)
+
+
+def test_two_streams_at_once(gpu):
+    """Calls that overlap on two streams, each with its own workspace, give what they give alone."""
+    announce("moe_experts and moe_route: two streams")
+    a = [device(expert_inputs(t, 12, 3, 512, 256, torch.float16, t), gpu) for t in (300, 257)]
+    logits = [torch.randn((5000, 200), generator=gen(s)).to(gpu) for s in (1, 2)]
+    alone = [K.moe_experts(*v) for v in a], [K.moe_route(v, 6) for v in logits]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [], []
+    for _ in range(5):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[0].append((j, K.moe_experts(*a[j])))
+                got[1].append((j, K.moe_route(logits[j], 6)))
+    torch.cuda.synchronize()
+    for j, y in got[0]:
+        assert torch.equal(y, alone[0][j])
+    for j, (w, i) in got[1]:
+        assert torch.equal(w, alone[1][j][0]) and torch.equal(i, alone[1][j][1])
+
+
+@pytest.mark.parametrize("t", [1, 60])
+def test_a_run_of_all_four_recorded_twice(gpu, t):
+    """Route, experts, quantise and project, recorded as two HIP graphs and replayed between eager calls."""
+    announce(f"operators in a row, {t} tokens, two graphs")
+    e, k, h, i = 10, 3, 512, 256
+    w13, s13, w2, s2 = device((*e4m3_weight(1, e, 2 * i, h), *e4m3_weight(2, e, h, i)), gpu)
+    wp, sp = device(e4m3_weight(3, 272, h), gpu)
+
+    def block(x, logits):
+        weights, ids = K.moe_route(logits, k)
+        y = K.moe_experts(x, ids, weights, w13, s13, w2, s2)
+        return K.linear_fp8_x8(*K.quant_fp8(y), wp, sp, out_dtype=torch.float32)
+
+    def inputs(seed):
+        g = gen(seed)
+        return torch.randn((t, h), generator=g).half().to(gpu), torch.randn((t, e), generator=g).to(gpu)
+
+    x, logits = inputs(0)
+    block(x, logits)  # every kernel is loaded before the first recording
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = block(x, logits)
+        graphs.append((graph, out))
+    for seed in (1, 2, 3):
+        fresh = inputs(seed)
+        want = block(*fresh)
+        for graph, out in graphs:
+            x.copy_(fresh[0])
+            logits.copy_(fresh[1])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            block(*inputs(seed + 10))  # the program's own calls between the replays
+
+
+def test_wide_rows_past_32_bit_offsets(gpu):
+    """Rows of a buffer of more than 2^32 bytes: offsets in 64 bits."""
+    announce("quant_fp8, linear_fp8_x8, moe_experts and moe_route: rows 16 MiB apart")
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of free memory")
+    t, h = 300, 256
+    x = torch.randn((t, h), generator=gen(4)).half().to(gpu)
+    far = torch.empty((t, 1 << 23), dtype=torch.float16, device=gpu)
+    far[:, :h] = x
+    q, s = K.quant_fp8(x)
+    qf, sf = K.quant_fp8(far[:, :h])
+    assert torch.equal(q.view(torch.uint8), qf.view(torch.uint8)) and torch.equal(s, sf)
+    a = device(expert_inputs(t, 4, 2, h, 128, torch.float16, 8), gpu)
+    want = K.moe_experts(x, *a[1:])
+    assert torch.equal(K.moe_experts(far[:, :h], *a[1:]), want)
+    K.moe_experts(x, *a[1:], out=far[:, h:2 * h])
+    assert torch.equal(far[:, h:2 * h], want)
+    w, i = K.moe_route(x, 8)
+    wf, i_f = K.moe_route(far[:, :h], 8)
+    assert torch.equal(w, wf) and torch.equal(i, i_f)
+    wp, sp = device(e4m3_weight(6, 64, h), gpu)
+    y = K.linear_fp8_x8(q, s, wp, sp)
+    K.linear_fp8_x8(q, s, wp, sp, out=far[:, :64])
+    assert torch.equal(far[:, :64], y)
+    q8 = far.view(torch.uint8)[:, 2048:2048 + h]
+    q8.copy_(q.view(torch.uint8))
+    if q8.stride(0) <= 1 << 23:
+        assert torch.equal(K.linear_fp8_x8(q8, s, wp, sp), y)
+    else:
+        with pytest.raises(RuntimeError, match="8 MiB"):
+            K.linear_fp8_x8(q8, s, wp, sp)

@@ -145,3 +145,17 @@ def test_tensors_off_the_gpu_are_refused() -> None:
         K.moe_experts(torch.zeros((2, 128)), torch.zeros((2, 1), dtype=torch.int32), torch.zeros((2, 1)),
                       torch.zeros((1, 256, 128), dtype=torch.float8_e4m3fn), torch.ones((1, 2, 1)),
                       torch.zeros((1, 128, 128), dtype=torch.float8_e4m3fn), torch.ones((1, 1, 1)))
+
+
+def test_block_refusals() -> None:
+    from router_ia.moe_block import MoeBlock, MoeLayerWeights
+
+    z = torch.zeros
+    w = MoeLayerWeights(z(128), z(5, 128), z(5, 256, 128), z(5, 2, 1), z(5, 128, 128), z(5, 1, 1), True)
+    with pytest.raises(ValueError, match="top_k"):
+        MoeBlock([w], 5)
+    block = MoeBlock([w], 4)
+    with pytest.raises(ValueError, match="fp32"):
+        block(0, z((2, 128), dtype=torch.float16))
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        block(0, z((2, 128)))
