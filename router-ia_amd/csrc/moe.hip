@@ -364,6 +364,7 @@ __device__ __forceinline__ void plan_place(const PlanArgs& a, int block, PlanSha
       if (a.blocks == 1) {
         total[j] = s.count[x];
       } else {
+#pragma unroll 8
         for (int b = 0; b < a.blocks; ++b) {
           const int c = a.counts[b * a.experts + x];
           before[j] += b < block ? c : 0;

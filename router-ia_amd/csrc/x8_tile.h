@@ -236,7 +236,9 @@ __device__ __forceinline__ void store_four(const X8Args& a, int64_t o, const f32
   }
 }
 
-// Eight results of a row at element o.  a.vec: rows and base allow whole-vector stores.
+// Eight results of a row at element o.  a.vec: rows and base allow whole-vector
+// stores.  STREAM: 16-bit results past the caches, where they outgrow them.
+template <bool STREAM = false>
 __device__ __forceinline__ void store_eight(const X8Args& a, int64_t o, const float (&v)[8]) {
   if (a.y_add) {  // fp32
     float* yp = static_cast<float*>(a.y) + o;
@@ -265,7 +267,11 @@ __device__ __forceinline__ void store_eight(const X8Args& a, int64_t o, const fl
     for (int i = 0; i < 4; ++i)
       w[i] = a.y_dtype == RIA_DT_F16 ? Kv16<RIA_DT_F16>::pack2(v[2 * i], v[2 * i + 1])
                                      : Kv16<RIA_DT_BF16>::pack2(v[2 * i], v[2 * i + 1]);
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.y) + o) = u32x4{w[0], w[1], w[2], w[3]};
+    u32x4* yp = reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.y) + o);
+    if constexpr (STREAM)
+      __builtin_nontemporal_store(u32x4{w[0], w[1], w[2], w[3]}, yp);
+    else
+      *yp = u32x4{w[0], w[1], w[2], w[3]};
   }
 }
 
@@ -529,7 +535,7 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
           const int rr = (wt * WT + t) * 32 + r, n = n0 + (wf * WF + f0) * 32 + c;
           if (rr >= rows || n >= a.n) continue;  // n is a multiple of 16: eight features are in or out
           const int64_t row = MODE == kX8Down ? a.order[first + rr] : first + rr;
-          store_eight(a, row * a.y_stride + n, v);
+          store_eight<(BM == 256)>(a, row * a.y_stride + n, v);
         }
       }
     }
