@@ -39,14 +39,36 @@ struct RouteArgs {
 // Unsigned integers in the order of floating values: 0 for a taken or absent
 // expert, -inf above it, NaN above every number; -0 ranks as 0.
 __device__ __forceinline__ uint32_t order_key(float v) {
-  if (v != v) return 0xffffffffu;
-  const uint32_t b = __float_as_uint(v == 0.f ? 0.f : v);
-  return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
+  const int32_t b = __float_as_int(v == 0.f ? 0.f : v);
+  const uint32_t o = static_cast<uint32_t>(b ^ (b >> 31 | static_cast<int32_t>(0x80000000u)));
+  return v != v ? 0xffffffffu : o;
 }
 __device__ __forceinline__ uint64_t order_key(double v) {
-  if (v != v) return ~uint64_t(0);
-  const uint64_t b = static_cast<uint64_t>(__double_as_longlong(v == 0.0 ? 0.0 : v));
-  return b ^ (b >> 63 ? ~uint64_t(0) : uint64_t(1) << 63);
+  const int64_t b = __double_as_longlong(v == 0.0 ? 0.0 : v);
+  const uint64_t o = static_cast<uint64_t>(b ^ (b >> 63 | INT64_MIN));
+  return v != v ? ~uint64_t(0) : o;
+}
+
+// V consecutive logits of a token from expert i0 on, -inf past the last.  No
+// load is in a branch (each would be waited for at its join): past the last
+// expert the last ones are loaded again.
+template <int XT, int V>
+__device__ __forceinline__ void load_logits(const RouteArgs& a, int64_t t, int i0, float (&x)[V]) {
+  const float ninf = -__builtin_inff();
+  if (V % 4 == 0 && a.vec) {  // whole groups of four, aligned
+#pragma unroll
+    for (int v = 0; v < V; v += 4) {
+      float f[4];
+      load_act4<XT>(a.logits, t * a.stride + min(i0 + v, a.experts - 4), f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[(v + i) % V] = f[i];
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = load_act<XT>(a.logits, t * a.stride + min(i0 + v, a.experts - 1));
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) x[v] = i0 + v < a.experts ? x[v] : ninf;
 }
 
 // The value behind an fp32 key.
@@ -112,136 +134,207 @@ __device__ __forceinline__ float exp_diff(float a, float b) {
   return expf(d) * (1.f + (lost == lost ? lost : 0.f));
 }
 
-// One wave per token, lane l holding experts V l .. V l + V - 1, so that of equal
-// choices the lowest lane has the lowest index.  WIDE: choices are scores in 64
-// bits (with a bias unlike scores come within an fp32 rounding of each other,
-// and the ids have to be the formula's).  Otherwise scores grow with the
-// logits, which are compared themselves.
-template <int XT, int V, bool WIDE>
-__global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const RouteArgs a) {
-  using Key = std::conditional_t<WIDE, uint64_t, uint32_t>;
-  __shared__ Key group_s[WIDE ? kRouteWaves : 1][WIDE ? 64 * V : 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t = (int64_t)blockIdx.x * kRouteWaves + wave;
-  if (t >= a.tokens) return;
+// sigmoid(x) exp(-min(m0, 0)), m0 the largest chosen logit: a common factor that
+// renormalising takes out again, and that keeps the scores of very negative
+// logits from vanishing.
+__device__ __forceinline__ float sigmoid_from(float x, float m0) {
+  const float c = m0 < 0.f ? m0 : 0.f;
+  return x > 0.f ? 1.f / (1.f + expf(-x)) : exp_diff(x, c) / (1.f + expf(x));
+}
+
+// The slot of the expert that every token visits.
+template <int XT>
+__device__ __forceinline__ void route_shared(const RouteArgs& a, int64_t t) {
+  const float l = load_act<XT>(a.logits, t * a.stride + a.experts);
+  a.weights[t * a.w_stride + a.top_k] = 1.f / (1.f + expf(-l));
+  a.ids[t * a.id_stride + a.top_k] = l == -__builtin_inff() ? -1 : a.experts;
+}
+
+// Largest over each row of 16 lanes.
+template <typename T>
+__device__ __forceinline__ T row_max(T v) {
+  v = max(v, lane_xor<8>(v));
+  v = max(v, lane_xor<4>(v));
+  v = max(v, lane_xor<2>(v));
+  return max(v, lane_xor<1>(v));
+}
+
+// Scores that grow with the logits, no groups, up to 256 experts and 16 of them
+// chosen: four tokens a wave, 16 lanes each, lane l holding experts V l .. V l +
+// V - 1 of its token.  A key is a logit's order with the expert's complement
+// below it (32 bits where the logits have 16, else 64), so no two are equal and
+// the lowest index wins ties by itself.  Each lane sorts its keys (an odd-even
+// merge network: no branches), and the token's best is then the largest of 16
+// heads, top_k times.  Against one wave per token and the best of all keys each
+// time, which waits on its lane exchanges: 16384 tokens, 8 of 256, 15.1 us in
+// the kernel, now 6.8 (instructions; the logits' 8.4 MB take 1.6).
+template <int XT, int V, int KM>
+__global__ __launch_bounds__(64 * kRouteWaves) void moe_route_rows_kernel(const RouteArgs a) {
+  constexpr bool kNarrow = XT != RIA_DT_F32;
+  constexpr int kLow = XT == RIA_DT_BF16 ? 16 : XT == RIA_DT_F16 ? 13 : 32;  // bits of a key below the logit's
+  constexpr int kList = KM < V ? KM : V;                                      // a lane's keys that can be taken
+  using Key = std::conditional_t<kNarrow, uint32_t, uint64_t>;
+  constexpr Key kMask = (Key(1) << kLow) - 1;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
+  const int64_t row = ((int64_t)blockIdx.x * kRouteWaves + wave) * 4 + (lane >> 4);
+  const int64_t t = min(row, (int64_t)a.tokens - 1);  // rows past the last repeat it, and store nothing
   const int e = a.experts;
   const float ninf = -__builtin_inff();
   float x[V];
-  if (V % 4 == 0 && a.vec) {  // whole groups of four, aligned
-#pragma unroll
-    for (int v = 0; v < V; v += 4) {
-      float f[4] = {ninf, ninf, ninf, ninf};
-      if (lane * V + v < e) load_act4<XT>(a.logits, t * a.stride + lane * V + v, f);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[(v + i) % V] = f[i];
-    }
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) x[v] = lane * V + v < e ? load_act<XT>(a.logits, t * a.stride + lane * V + v) : ninf;
-  }
-  // the softmax's largest logit (NaN if there is one), and in WIDE its normaliser
-  float top = 0.f;
-  double total = 1.0;
-  if (!a.sigmoid && (WIDE || !a.renorm)) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v) m = max(m, order_key(x[v]));
-    m = wave_max(m);
-    top = key_value(m);
-    if (top == ninf) top = 0.f;
-    if constexpr (WIDE) {
-      double s = 0.0;
-#pragma unroll
-      for (int v = 0; v < V; ++v) s += exp(static_cast<double>(x[v]) - static_cast<double>(top));
-      total = wave_sum64(s);
-    } else {
-      float s = 0.f;
-#pragma unroll
-      for (int v = 0; v < V; ++v) s += exp_diff(x[v], top);
-      total = static_cast<double>(wave_sum(s));
-    }
-    if (total == 0.0) total = 1.0;
-  }
+  load_logits<XT, V>(a, t, l16 * V, x);
+  auto top_bits = [](uint32_t o) { return kNarrow ? static_cast<Key>(o >> kLow % 32 << kLow % 32) : static_cast<Key>(o) << kLow % 64; };
   Key key[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int i = lane * V + v;
-    if constexpr (WIDE) {
-      double c = x[v];
-      if (i < e && x[v] != ninf) {
-        const double l = x[v];
-        c = (a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - static_cast<double>(top)) / total) +
-            (a.bias ? static_cast<double>(a.bias[i]) : 0.0);
-      }
-      key[v] = i < e ? order_key(c) : 0;
-    } else {
-      key[v] = i < e ? order_key(x[v]) : 0;
-    }
+    const int i = l16 * V + v;
+    const Key k = top_bits(order_key(x[v])) | (kMask - static_cast<Key>(i));
+    key[v] = i < e ? k : 0;
   }
-  const Key none = WIDE ? static_cast<Key>(order_key(-__builtin_inf())) : static_cast<Key>(order_key(ninf));
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < V; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const Key lo = min(key[i + j], key[i + j + k]);
+            key[i + j] = max(key[i + j], key[i + j + k]);
+            key[i + j + k] = lo;
+          }
+  Key mine = 0, first = 0;
+  for (int j = 0; j < a.top_k; ++j) {
+    const Key best = row_max(key[0]);
+    const bool taken = key[0] == best;
+#pragma unroll
+    for (int v = 0; v + 1 < kList; ++v) {  // (values, not elements, to choose from: no index of the lane's own)
+      const Key here = key[v], next = key[v + 1];
+      key[v] = taken ? next : here;
+    }
+    key[kList - 1] = taken ? 0 : key[kList - 1];
+    if (j == 0) first = best;
+    if (l16 == j) mine = best;
+  }
+  auto value = [&](Key k) {  // the logit of a key
+    uint32_t o = static_cast<uint32_t>(kNarrow ? k >> kLow % 32 << kLow % 32 : k >> kLow % 64);
+    if (kNarrow && !(o >> 31)) o |= static_cast<uint32_t>(kMask);  // a negative one's zeros are ones in its order
+    return key_value(o);
+  };
+  const Key none = top_bits(order_key(ninf)) | kMask;
+  const bool chosen = mine > none;
+  const float my_x = chosen ? value(mine) : ninf;
+  const float m0 = first > none ? value(first) : 0.f;  // the largest logit, NaN if there is one
+  float w = 0.f;
+  if (a.renorm) {
+    if (chosen) w = a.sigmoid ? sigmoid_from(my_x, m0) : exp_diff(my_x, m0);
+    float sum = add_xor<8>(w);
+    sum = add_rn(sum, __uint_as_float(lane_xor<4>(__float_as_uint(sum))));
+    sum = add_xor<1>(add_xor<2>(sum));
+    if (sum != 0.f) w = w / sum;
+  } else if (a.sigmoid) {
+    if (chosen) w = 1.f / (1.f + expf(-my_x));
+  } else {
+    float sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum += exp_diff(x[v], m0);
+    sum = add_xor<8>(sum);
+    sum = add_rn(sum, __uint_as_float(lane_xor<4>(__float_as_uint(sum))));
+    sum = add_xor<1>(add_xor<2>(sum));
+    if (chosen) w = exp_diff(my_x, m0) / sum;
+  }
+  if (row >= a.tokens) return;
+  if (l16 < a.top_k) {
+    a.weights[t * a.w_stride + l16] = w * a.scale;
+    a.ids[t * a.id_stride + l16] = chosen ? static_cast<int>(kMask - (mine & kMask)) : -1;
+  }
+  if (a.shared && l16 == 15) route_shared<XT>(a, t);
+}
+
+// Whether two fp32 choices lie too near for their order to be sure: scores are
+// within 2^-20.5 of the formula's (exp to 3 ulps, a sum of up to 1024 terms), a
+// sum of two and the compared other add up to 2^-18.5, roundings of the choices
+// themselves to 2^-22 of them.
+__device__ __forceinline__ bool unsure(uint32_t a, uint32_t b) {
+  const float x = key_value(a), y = key_value(b);
+  return !(fabsf(x - y) > 0x1p-18f * (1.f + fabsf(x)));
+}
+__device__ __forceinline__ bool unsure(uint64_t, uint64_t) { return false; }
+__device__ __forceinline__ float key_sum(uint32_t a, uint32_t b) { return key_value(a) + key_value(b); }
+__device__ __forceinline__ double key_sum(uint64_t a, uint64_t b) {
+  auto value = [](uint64_t k) {
+    const double v = __longlong_as_double(static_cast<int64_t>(k ^ (k >> 63 ? uint64_t(1) << 63 : ~uint64_t(0))));
+    return k == ~uint64_t(0) ? __builtin_nan("") : v;
+  };
+  return value(a) + value(b);
+}
+
+// One token's groups and top_k from the keys of its choices, lane l holding
+// experts V l .. V l + V - 1, so that of equal choices the lowest lane has the
+// lowest index.  Lane j gets the j-th expert and its logit.  GUARD (fp32 keys of
+// scores): false where the outcome hangs on choices that are too near.
+template <typename Key, int V, bool GUARD>
+__device__ __forceinline__ bool route_select(const RouteArgs& a, int lane, Key (&key)[V], const float (&x)[V], Key* s,
+                                             int& my_id, float& my_x) {
+  const int e = a.experts;
+  const Key none = static_cast<Key>(order_key(std::conditional_t<sizeof(Key) == 8, double, float>(-__builtin_inff())));
+  bool sure = true;
   if (a.groups > 1) {
-    // rank of a group: its best key, or in WIDE with top2 the sum of its best two
     const int per = e / a.groups;
-    Key rank = 0;  // lane g: group g's
-    if constexpr (WIDE) {
-      Key* s = group_s[wave];
 #pragma unroll
-      for (int v = 0; v < V; ++v) s[lane * V + v] = key[v];
-      __builtin_amdgcn_wave_barrier();
-      if (lane < a.groups) {
-        Key b0 = 0, b1 = 0;
-        for (int i = 0; i < per; ++i) {
-          const Key c = s[lane * per + i];
-          b1 = max(b1, min(b0, c));
-          b0 = max(b0, c);
-        }
-        rank = b0;
-        if (a.top2 && per > 1) {
-          auto value = [](Key k) {
-            return k == ~Key(0) ? __builtin_nan("")
-                                : __longlong_as_double(static_cast<int64_t>(k ^ (k >> 63 ? Key(1) << 63 : ~Key(0))));
-          };
-          rank = order_key(value(b0) + value(b1));
-        }
-      }
-    } else {
-      for (int g = 0; g < a.groups; ++g) {
-        Key m = 0;
+    for (int v = 0; v < V; ++v) s[lane * V + v] = key[v];
+    __builtin_amdgcn_wave_barrier();
+    Key b0 = 0, b1 = 0;  // lane g: group g's best two
+    const int base = min(lane, a.groups - 1) * per;
+    for (int i = 0; i < per; i += 4) {
+      Key c[4];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const int i = lane * V + v;
-          m = max(m, i >= g * per && i < (g + 1) * per ? key[v] : 0);
-        }
-        m = wave_max(m);
-        if (lane == g) rank = m;
+      for (int q = 0; q < 4; ++q) c[q] = s[base + min(i + q, per - 1)];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const Key k = i + q < per ? c[q] : 0;
+        b1 = max(b1, min(b0, k));
+        b0 = max(b0, k);
       }
     }
+    Key rank = a.top2 && per > 1 ? static_cast<Key>(order_key(key_sum(b0, b1))) : b0;
+    rank = lane < a.groups ? rank : 0;
     int better = 0;  // groups that come before this one
     for (int j = 0; j < a.groups; ++j) {
       Key o;
-      if constexpr (WIDE)
+      if constexpr (sizeof(Key) == 8)
         o = static_cast<Key>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank >> 32), j))) << 32 |
             static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank), j));
       else
         o = static_cast<Key>(__builtin_amdgcn_readlane(static_cast<int>(rank), j));
       better += o > rank || (o == rank && j < lane);
     }
-    const uint64_t open = __ballot(lane < a.groups && better < a.top_groups);
+    const bool in = lane < a.groups && better < a.top_groups;
+    const uint64_t open = __ballot(in);
+    if constexpr (GUARD) {
+      const Key best_out = uniform(wave_max(in ? Key(0) : rank)), worst_in = uniform(~wave_max(in ? ~rank : Key(0)));
+      if (best_out > none && unsure(worst_in, best_out)) sure = false;
+    }
+    const float inv = 1.f / static_cast<float>(per);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const int i = lane * V + v;
-      if (i < e && !(open >> (i / per) & 1)) key[v] = 0;
+      const int g = static_cast<int>((static_cast<float>(lane * V + v) + 0.5f) * inv);  // (lane V + v) / per: both below 2^11
+      key[v] = open >> min(g, 63) & 1 ? key[v] : 0;
     }
   }
   // top_k times the best that is left; who holds it is scalar work, beside the other waves' vector work
-  int my_id = -1;
-  float my_x = ninf;
-  for (int j = 0; j < a.top_k; ++j) {
+  my_id = -1;
+  my_x = -__builtin_inff();
+  Key last = 0;
+  for (int j = 0; j < a.top_k + (GUARD ? 1 : 0); ++j) {
     Key head = key[0];
 #pragma unroll
     for (int v = 1; v < V; ++v) head = max(head, key[v]);
     const Key best = uniform(wave_max(head));
     if (best <= none) break;  // the slots left over keep id -1
+    if (GUARD && j > 0 && unsure(last, best)) sure = false;
+    if (GUARD && j == a.top_k) break;  // looked at only
+    last = best;
     uint64_t has[V], any = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) any |= has[v] = __ballot(key[v] == best);
@@ -249,21 +342,99 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
     int at = V - 1;
 #pragma unroll
     for (int v = V - 2; v >= 0; --v) at = has[v] >> from & 1 ? v : at;
-    float bx;
-    if constexpr (WIDE) {
-      bx = x[0];
+    float bx = x[0];
 #pragma unroll
-      for (int v = 1; v < V; ++v) bx = at == v ? x[v] : bx;
-      bx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(bx), from));
-    } else {
-      bx = key_value(best);
+    for (int v = 1; v < V; ++v) {
+      const float xv = x[v];
+      bx = at == v ? xv : bx;
     }
+    bx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(bx), from));
 #pragma unroll
-    for (int v = 0; v < V; ++v) key[v] = lane == from && at == v ? 0 : key[v];
+    for (int v = 0; v < V; ++v) {
+      const Key k = key[v];
+      key[v] = lane == from && at == v ? 0 : k;
+    }
     if (lane == j) {
       my_id = from * V + at;
       my_x = bx;
     }
+  }
+  return sure;
+}
+
+// One wave per token: groups, biases, many experts.  SCORED: choices are scores
+// (with a bias, or ranked by sums), which are compared in fp32 first; where
+// their order is not sure, which takes choices within some 2^-18 of each other,
+// the token is chosen again with scores in 64 bits, so that the ids are the
+// formula's.  Otherwise scores grow with the logits, which are compared
+// themselves.  256 experts in 8 groups with a bias: 16384 tokens 34 us, 41 in 64
+// bits throughout (65536: 101 and 145).  At 4099 tokens both take 16: some
+// tokens of a batch are chosen again, and 4 us of that show at the end.
+template <int XT, int V, bool SCORED>
+__global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const RouteArgs a) {
+  __shared__ uint64_t group_s[kRouteWaves][64 * V];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t t = (int64_t)blockIdx.x * kRouteWaves + wave;
+  if (t >= a.tokens) return;
+  const int e = a.experts;
+  const float ninf = -__builtin_inff();
+  float x[V];
+  load_logits<XT, V>(a, t, lane * V, x);
+  // the softmax's largest logit (NaN if there is one) and normaliser
+  float top = 0.f, total = 1.f;
+  if (!a.sigmoid && (SCORED || !a.renorm)) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) m = max(m, order_key(x[v]));
+    top = key_value(wave_max(m));
+    if (top == ninf) top = 0.f;
+    float s = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) s += exp_diff(x[v], top);
+    total = wave_sum(s);
+    if (total == 0.f) total = 1.f;
+  }
+  int my_id;
+  float my_x;
+  if constexpr (SCORED) {
+    float bias[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) bias[v] = a.bias ? a.bias[min(lane * V + v, e - 1)] : 0.f;
+    uint32_t key[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float p = a.sigmoid ? 1.f / (1.f + expf(-x[v])) : exp_diff(x[v], top) / total;
+      const float c = x[v] == ninf ? ninf : p + bias[v];
+      key[v] = lane * V + v < e ? order_key(c) : 0;
+    }
+    if (!route_select<uint32_t, V, true>(a, lane, key, x, reinterpret_cast<uint32_t*>(group_s[wave]), my_id, my_x)) {
+      double wide_total = 1.0;
+      if (!a.sigmoid) {
+        double s = 0.0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) s += exp(static_cast<double>(x[v]) - static_cast<double>(top));
+        wide_total = wave_sum64(s);
+        if (wide_total == 0.0) wide_total = 1.0;
+      }
+      uint64_t wide[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const double l = x[v];
+        const double p = a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - static_cast<double>(top)) / wide_total;
+        const double c = x[v] == ninf ? static_cast<double>(ninf) : p + static_cast<double>(bias[v]);
+        wide[v] = lane * V + v < e ? order_key(c) : 0;
+      }
+      __builtin_amdgcn_wave_barrier();
+      route_select<uint64_t, V, false>(a, lane, wide, x, group_s[wave], my_id, my_x);
+    }
+  } else {
+    uint32_t key[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const uint32_t k = order_key(x[v]);
+      key[v] = lane * V + v < e ? k : 0;
+    }
+    route_select<uint32_t, V, false>(a, lane, key, x, reinterpret_cast<uint32_t*>(group_s[wave]), my_id, my_x);
   }
   // the chosen scores (lanes 0 .. top_k - 1)
   float w = 0.f;
@@ -271,43 +442,45 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
     // about the largest chosen logit: the weights hold where every score underflows
     const uint32_t m = wave_max(my_id >= 0 ? order_key(my_x) : 0u);
     const float m0 = m == 0 ? 0.f : key_value(m);
-    if (my_id >= 0) {
-      if (!a.sigmoid) {
-        w = exp_diff(my_x, m0);
-      } else {  // sigmoid(x) exp(-c), c = min(m0, 0)
-        const float c = m0 < 0.f ? m0 : 0.f;
-        w = my_x > 0.f ? 1.f / (1.f + expf(-my_x)) : exp_diff(my_x, c) / (1.f + expf(my_x));
-      }
-    }
-    if (WIDE && !a.sigmoid && total != total) w = __builtin_nanf("");  // a NaN logit that was not chosen
+    if (my_id >= 0) w = a.sigmoid ? sigmoid_from(my_x, m0) : exp_diff(my_x, m0);
+    if (SCORED && !a.sigmoid && total != total) w = __builtin_nanf("");  // a NaN logit that was not chosen
     const float sum = wave_sum(w);
     if (sum != 0.f) w = w / sum;
   } else if (my_id >= 0) {
-    w = a.sigmoid ? 1.f / (1.f + expf(-my_x)) : static_cast<float>(static_cast<double>(exp_diff(my_x, top)) / total);
+    w = a.sigmoid ? 1.f / (1.f + expf(-my_x)) : exp_diff(my_x, top) / total;
   }
   if (lane < a.top_k) {
     a.weights[t * a.w_stride + lane] = w * a.scale;
     a.ids[t * a.id_stride + lane] = my_id;
   }
-  if (a.shared && lane == 63) {
-    const float l = load_act<XT>(a.logits, t * a.stride + e);
-    a.weights[t * a.w_stride + a.top_k] = 1.f / (1.f + expf(-l));
-    a.ids[t * a.id_stride + a.top_k] = l == ninf ? -1 : e;
-  }
+  if (a.shared && lane == 63) route_shared<XT>(a, t);
 }
 
-template <int XT, bool WIDE>
+template <int XT, bool SCORED>
 static void launch_route(const RouteArgs& a, hipStream_t st) {
+  if (!SCORED && a.groups == 1 && a.experts <= 256 && a.top_k <= 16) {
+    const dim3 grid((a.tokens + 4 * kRouteWaves - 1) / (4 * kRouteWaves)), block(64 * kRouteWaves);
+    const bool few = a.top_k <= 8;
+    if (a.experts <= 64)
+      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 4, 16>), grid, block, 0, st, a);
+    else if (a.experts <= 128 && few)
+      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 8, 8>), grid, block, 0, st, a);
+    else if (few)
+      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 16, 8>), grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 16, 16>), grid, block, 0, st, a);
+    return;
+  }
   const dim3 grid((a.tokens + kRouteWaves - 1) / kRouteWaves), block(64 * kRouteWaves);
   const int v = (a.experts + 63) / 64;
   if (v <= 1)
-    hipLaunchKernelGGL((moe_route_kernel<XT, 1, WIDE>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((moe_route_kernel<XT, 1, SCORED>), grid, block, 0, st, a);
   else if (v <= 4)
-    hipLaunchKernelGGL((moe_route_kernel<XT, 4, WIDE>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((moe_route_kernel<XT, 4, SCORED>), grid, block, 0, st, a);
   else if (v <= 8)
-    hipLaunchKernelGGL((moe_route_kernel<XT, 8, WIDE>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((moe_route_kernel<XT, 8, SCORED>), grid, block, 0, st, a);
   else
-    hipLaunchKernelGGL((moe_route_kernel<XT, 16, WIDE>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((moe_route_kernel<XT, 16, SCORED>), grid, block, 0, st, a);
 }
 
 // ----------------------------------------------------------------------------- experts
@@ -816,11 +989,11 @@ extern "C" int ria_moe_route(int tokens, int experts, int top_k, const void* log
                     top_groups, group_score == RIA_ROUTE_GROUP_TOP2, renormalize != 0, s, scale, weights,
                     weights_row_stride, ids, ids_row_stride, vec};
   // scores need comparing where a bias or a sum of two stands between them and the logits
-  const bool wide = bias || (num_groups > 1 && group_score == RIA_ROUTE_GROUP_TOP2);
+  const bool scored = bias || (num_groups > 1 && group_score == RIA_ROUTE_GROUP_TOP2);
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto launch = [&](auto dt) {
     constexpr int XT = decltype(dt)::value;
-    if (wide)
+    if (scored)
       launch_route<XT, true>(a, st);
     else
       launch_route<XT, false>(a, st);
