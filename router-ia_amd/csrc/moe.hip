@@ -718,7 +718,6 @@ __global__ __launch_bounds__(256) void moe_up_pairs_kernel(const PairsArgs a) {
 // 16 features of one token's sum, a wave for each slot (in turns of
 // kSumWaves); the terms meet in LDS and are added in slot order.
 constexpr int kSumWaves = 8;
-template <int DT>
 __global__ __launch_bounds__(64 * kSumWaves) void moe_down_pairs_kernel(const PairsArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t h_s[kSumWaves][kFewChunk];
   __shared__ float hs_s[kSumWaves][kFewChunk / kX8Block];
@@ -770,7 +769,7 @@ __global__ __launch_bounds__(64 * kSumWaves) void moe_down_pairs_kernel(const Pa
     if ((lane & 15) == 0) {  // column 0: every column is the pair's
       const float pw = some ? a.pair_w[(int64_t)t * a.pair_w_stride + j] : 0.f;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) term[wave][4 * (lane >> 4) + q] = some ? through_dtype<DT>(pw * acc[q]) : 0.f;
+      for (int q = 0; q < 4; ++q) term[wave][4 * (lane >> 4) + q] = some ? pw * acc[q] : 0.f;
     }
     __syncthreads();
     if (tid < 16)
@@ -785,7 +784,8 @@ __global__ __launch_bounds__(64 * kSumWaves) void moe_down_pairs_kernel(const Pa
 }
 
 struct CombineArgs {
-  const void* slots;  // [tokens * top_k, hidden], in x's dtype
+  const void* slots;  // [tokens * top_k, hidden]: fp32, or fp16 times 2^(e - 127)
+  const uint8_t* slot_e;  // e [tokens * top_k, hidden / 64]
   const int32_t* ids;
   int64_t id_stride;
   int tokens, top_k, experts, hidden;
@@ -815,7 +815,15 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs a) {
       const int e = j0 + j < a.top_k ? a.ids[t * a.id_stride + j0 + j] : -1;
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[j][i] = 0.f;
-      if (e >= 0 && e < a.experts) load_act8<DT>(a.slots, (t * a.top_k + j0 + j) * a.hidden + c, v[j]);
+      if (e >= 0 && e < a.experts) {
+        const int64_t pair = t * a.top_k + j0 + j;
+        load_act8<DT>(a.slots, pair * a.hidden + c, v[j]);
+        if constexpr (DT != RIA_DT_F32) {
+          const float scale = x8_scale(a.slot_e[pair * (a.hidden / 64) + c / 64]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[j][i] *= scale;
+        }
+      }
     }
 #pragma unroll
     for (int j = 0; j < kCombineAhead; ++j)
@@ -850,16 +858,24 @@ static bool moe_by_pairs(int64_t pairs, int experts, int hidden, int inter) {
   return (pairs - met) * 3.0 * hidden * inter <= 40e6;
 }
 
-// Pairs of one expert that a tile takes.  256 from 192 pairs an expert on,
-// where full tiles outweigh what the last ones leave empty: (256, 8, 2048, 512)
-// 2048 tokens 243 us in tiles of 64, 300 of 256, 4096 tokens 338 and 357, 8192
-// tokens 564 and 533.  (fp32 x has no kernel of 256.)
+// Whether most experts' pairs fill one tile: the time is the weights' then.  They
+// are read once and kept in no cache (a pure read of 512 MB: 5.8 TB/s, 6.5 past
+// the caches), and widened for the products, which costs next to nothing beside
+// the reading: (256, 8, 2048, 512) 128 tokens 140 us, 144 in e4m3 products, 158
+// through the caches; 1024 tokens 189, 182 and 204.
+static bool moe_once(int64_t pairs, int experts) { return pairs <= (int64_t)experts * 32; }
+
+// Pairs of one expert that a tile takes.  Same sizes, tiles of 32 / 64: 128
+// tokens 140 / 157 us, 512 tokens 159 / 169, 768 tokens 184 / 182; of 64 / 256:
+// 2048 tokens 243 / 300, 4096 tokens 338 / 357, 8192 tokens 564 / 533.  (fp32 x
+// has no kernel of 256.)
 static int moe_tile(int64_t pairs, int experts, int x_dtype) {
+  if (pairs <= (int64_t)experts * 16) return 32;
   return x_dtype != RIA_DT_F32 && pairs >= (int64_t)experts * 192 ? 256 : 64;
 }
 
 struct MoeLayout {
-  int64_t x8, xs, counts, order, tiles, ntiles, act, h8, hs, slots, bytes;
+  int64_t x8, xs, counts, order, tiles, ntiles, act, h8, hs, slots, slot_e, bytes;
 };
 static MoeLayout moe_layout(int64_t tokens, int top_k, int experts, int hidden, int inter, int x_dtype) {
   MoeLayout l{};
@@ -882,6 +898,7 @@ static MoeLayout moe_layout(int64_t tokens, int top_k, int experts, int hidden, 
     l.h8 = take(pairs * inter);
     l.hs = take(pairs * (inter / kX8Block) * 4);
     l.slots = take(pairs * hidden * (x_dtype == RIA_DT_F32 ? 4 : 2));
+    l.slot_e = take(x_dtype == RIA_DT_F32 ? 0 : pairs * (hidden / 64));
   }
   l.bytes = at;
   return l;
@@ -907,18 +924,16 @@ static void launch_moe_tiles(const ria_moe_experts_desc& d, const MoeLayout& l, 
   up.h8 = static_cast<uint8_t*>(at(l.h8));
   up.hs = static_cast<float*>(at(l.hs));
   up.m = d.tokens;
-  const bool wide = d.x_dtype == RIA_DT_F32;
-  // most experts' pairs fill one tile: their weights are read once, and kept in no cache
-  const bool once = (int64_t)d.tokens * d.top_k <= (int64_t)d.experts * 32;
+  const bool wide = d.x_dtype == RIA_DT_F32, once = moe_once((int64_t)d.tokens * d.top_k, d.experts);
   auto grid_of = [&](int feature_tiles) { return dim3(static_cast<unsigned>((most * feature_tiles + 7) / 8 * 8)); };
-  if (wide && once)
+  if (tile == 32)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 1, 4, 1, true, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
+  else if (once)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   else if (wide)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   else if (tile == 256)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 4, 2, 2, 4, false>), grid_of(d.inter / 128), dim3(512), 0, st, up);
-  else if (once)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   else
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   X8Args dn = up;
@@ -932,18 +947,20 @@ static void launch_moe_tiles(const ria_moe_experts_desc& d, const MoeLayout& l, 
   dn.k = d.inter;
   dn.y = at(l.slots);
   dn.y_stride = d.hidden;
-  dn.y_dtype = d.x_dtype;
+  dn.y_dtype = wide ? RIA_DT_F32 : RIA_DT_F16;
+  dn.ye = static_cast<uint8_t*>(at(l.slot_e));
+  dn.ye_stride = d.hidden / 64;
   dn.vec = 1;
   dn.pair_w = d.weights;
   dn.pair_w_stride = d.weights_row_stride;
-  if (wide && once)
+  if (tile == 32)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 1, true, true>), grid_of(d.hidden / 128), dim3(128), 0, st, dn);
+  else if (once)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, true, true>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
   else if (wide)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, true>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
   else if (tile == 256)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 4, 2, 2, 4, false>), grid_of((d.hidden + 255) / 256), dim3(512), 0, st, dn);
-  else if (once)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, false, true>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
   else
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, false>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
 }
@@ -1052,12 +1069,7 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
       hipLaunchKernelGGL((moe_up_pairs_kernel<RIA_DT_F16>), ugrid, dim3(256), lds, st, p);
     else
       hipLaunchKernelGGL((moe_up_pairs_kernel<RIA_DT_F32>), ugrid, dim3(256), lds, st, p);
-    if (d->x_dtype == RIA_DT_BF16)
-      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_BF16>), dgrid, dim3(64 * kSumWaves), 0, st, p);
-    else if (d->x_dtype == RIA_DT_F16)
-      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_F16>), dgrid, dim3(64 * kSumWaves), 0, st, p);
-    else
-      hipLaunchKernelGGL((moe_down_pairs_kernel<RIA_DT_F32>), dgrid, dim3(64 * kSumWaves), 0, st, p);
+    hipLaunchKernelGGL(moe_down_pairs_kernel, dgrid, dim3(64 * kSumWaves), 0, st, p);
     return check_launch(who);
   }
   const int tile = moe_tile(pairs, d->experts, d->x_dtype);
@@ -1079,15 +1091,13 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
     hipLaunchKernelGGL((moe_prepare_kernel<RIA_DT_F32>), pgrid, dim3(256), 0, st, plan, quant);
   if (plan.blocks > 1) hipLaunchKernelGGL(moe_place_kernel, dim3(plan.blocks), dim3(256), 0, st, plan);
   launch_moe_tiles(*d, l, most, tile, st);
-  const CombineArgs c{at(l.slots), d->ids, d->ids_row_stride, d->tokens, d->top_k, d->experts, d->hidden, d->out,
+  const CombineArgs c{at(l.slots), static_cast<const uint8_t*>(at(l.slot_e)), d->ids, d->ids_row_stride, d->tokens, d->top_k, d->experts, d->hidden, d->out,
                       d->out_dtype, d->out_row_stride, d->accumulate != 0,
                       reinterpret_cast<uintptr_t>(d->out) % 16 == 0 && d->out_row_stride % 8 == 0};
   const dim3 grid(static_cast<unsigned>(((int64_t)d->tokens * (d->hidden / 8) + 255) / 256));
-  if (d->x_dtype == RIA_DT_BF16)
-    hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_BF16>), grid, dim3(256), 0, st, c);
-  else if (d->x_dtype == RIA_DT_F16)
-    hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F16>), grid, dim3(256), 0, st, c);
-  else
+  if (d->x_dtype == RIA_DT_F32)
     hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F32>), grid, dim3(256), 0, st, c);
+  else
+    hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F16>), grid, dim3(256), 0, st, c);
   return check_launch(who);
 }

@@ -127,6 +127,14 @@ __device__ __forceinline__ float x8_swiglu(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f)) * u;
 }
 
+// Biased exponent of the scale of a slot's 64 terms whose largest finite |y| is
+// top: the largest becomes 2^14 to 2^15, so fp16 keeps 11 bits of every term
+// down to 2^-28 of it, whatever the range of x's type.
+__device__ __forceinline__ uint32_t term_scale_exp(float top) {
+  const uint32_t u = __float_as_uint(top);
+  return u == 0 ? 127u : static_cast<uint32_t>(max(static_cast<int>(u >> 23) - 14, 1));
+}
+
 // Eight values of a block to e4m3 at d; the first of its 16 lanes stores the scale.
 __device__ __forceinline__ void quant_eight(float (&v)[8], uint8_t* d, float* s, int lane) {
   float top = 0.f;
@@ -190,6 +198,8 @@ struct X8Args {
   int top_k;
   const float* pair_w;
   int64_t pair_w_stride;
+  uint8_t* ye;       // kX8Down with RIA_DT_F16: y holds term / 2^(e - 127), e [pairs, ye_stride] one per 64 features
+  int ye_stride;
   uint8_t* h8;       // kX8Up: [positions, n / 2] e4m3 and its scales [positions, n / 256]
   float* hs;
 };
@@ -517,13 +527,32 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
       }
 #pragma unroll
       for (int f0 = 0; f0 < WF; f0 += 2) {
+        float scale = pw;
+        if constexpr (MODE == kX8Down) {
+          if (a.y_dtype != RIA_DT_F32) {
+            float top = 0.f;
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) top = fmaxf(top, finite_abs(pw * acc[f0 + f][t][i]));
+            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            const uint32_t e = term_scale_exp(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
+            scale = x8_inverse(e);
+            const int rr = (wt * WT + t) * 32 + l32, g = (n0 + (wf * WF + f0) * 32) / 64;
+            if (half == 0 && rr < rows && g < a.ye_stride)
+              a.ye[(int64_t)a.order[first + rr] * a.ye_stride + g] = static_cast<uint8_t>(e);
+          } else {
+            scale = 1.f;
+          }
+        }
 #pragma unroll
         for (int f = 0; f < 2; ++f)
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             f32x4 v;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = MODE == kX8Down ? pw * acc[f0 + f][t][4 * q + i] : acc[f0 + f][t][4 * q + i];
+            for (int i = 0; i < 4; ++i)
+              v[i] = MODE == kX8Down ? pw * acc[f0 + f][t][4 * q + i] * scale : acc[f0 + f][t][4 * q + i];
             *reinterpret_cast<f32x4*>(st + l32 * kPitch + f * 32 + 8 * q + 4 * half) = v;
           }
 #pragma unroll

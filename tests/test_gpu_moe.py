@@ -9,6 +9,7 @@ their order, n * 2^-24 of the sum of the terms' magnitudes at most.
 from __future__ import annotations
 
 import math
+from typing import NamedTuple
 
 import pytest
 import torch
@@ -85,21 +86,28 @@ def route64(logits, k, scoring="softmax", bias=None, num_groups=1, top_groups=1,
     return torch.tensor(out_w, dtype=torch.float64), torch.tensor(out_i, dtype=torch.int32)
 
 
+class Mags(NamedTuple):
+    terms: torch.Tensor
+    products: torch.Tensor
+
+
 def experts64(x, ids, weights, w13, s13, w2, s2):
-    """The sum over the slots, and the sum of the slots' magnitudes (for the tolerance)."""
+    """The sum over the slots and, for the tolerance, Mags: of the slots' terms, and of the products they sum."""
     e, i = w13.shape[0], w2.shape[2]
     xq = rows64(*quant64(x))
     out = torch.zeros(x.shape, dtype=torch.float64)
-    mag = torch.zeros_like(out)
+    mag = Mags(torch.zeros_like(out), torch.zeros_like(out))
     for j in range(e):
         rows, slot = torch.nonzero(ids == j, as_tuple=True)
         if rows.numel() == 0:
             continue
         z = xq[rows] @ widen(w13[j], s13[j]).T
         a = z[:, :i] * torch.sigmoid(z[:, :i]) * z[:, i:]
-        term = rows64(*quant64(a)) @ widen(w2[j], s2[j]).T * weights[rows, slot].double()[:, None]
+        aq, down, pw = rows64(*quant64(a)), widen(w2[j], s2[j]).T, weights[rows, slot].double()[:, None]
+        term = aq @ down * pw
         out.index_add_(0, rows, term)
-        mag.index_add_(0, rows, term.abs())
+        mag.terms.index_add_(0, rows, term.abs())
+        mag.products.index_add_(0, rows, aq.abs() @ down.abs() * pw.abs())
     return out, mag
 
 
@@ -305,7 +313,7 @@ def test_route_extreme_logits(gpu):
 EXPERTS = [  # (tokens, experts, top_k, hidden, inter)
     (1, 8, 2, 256, 128), (1, 16, 8, 2048, 512), (2, 4, 1, 128, 128), (3, 5, 5, 384, 256), (7, 16, 3, 512, 640),
     (17, 3, 2, 256, 128), (40, 33, 4, 256, 384), (130, 6, 2, 640, 256), (200, 2, 2, 256, 128), (300, 40, 6, 512, 128),
-    (700, 3, 2, 256, 256), (2100, 5, 2, 256, 128),
+    (700, 3, 2, 256, 256), (2100, 5, 2, 256, 128), (400, 20, 1, 384, 256), (900, 24, 2, 640, 128),
 ]
 
 
@@ -319,15 +327,19 @@ def expert_inputs(t, e, k, h, i, dtype, seed):
     return x, ids, weights, w13, s13, w2, s2
 
 
-def expert_tolerance(out, mag, k, dtype, slack):
+def expert_tolerance(out, mag, i, dtype, slack):
     """Roundings of the slots' terms and of the sum to out's type, and the fp32 sums' own.
+
+    Terms are kept to 11 bits or more, or in out's type's step; a sum of i
+    products in fp32, its scalings and the sum over the slots are off by at
+    most (i + 16) 2^-24 of the products' magnitudes.
 
     The hidden values are e4m3: where an fp32 sum of another order lies on the
     other side of a rounding border, one value moves by a step, 2^-3 of itself
     at most.  `slack` bounds what such moves add, relative to the row's size.
     """
     size = out.abs().amax(-1, keepdim=True)
-    return half_step(dtype) * (out.abs() + mag) + 1e-5 * mag + slack * size
+    return half_step(dtype) * (out.abs() + mag.terms) + (i + 16) * 2.0 ** -24 * mag.products + slack * size
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
@@ -345,13 +357,13 @@ def test_experts_match_definition(gpu, t, e, k, h, i, dtype):
         assert not bool(out[1].any())
     # one value of `i` moved by 2^-3 of itself changes a term by 2^-3 / sqrt(i) of its size, typically;
     # the largest values are 4 sigma, and two may move in a row
-    err, tol = (out - want).abs(), expert_tolerance(want, mag, k, dtype, 0.125 * 4 * 2 / math.sqrt(i))
+    err, tol = (out - want).abs(), expert_tolerance(want, mag, i, dtype, 0.125 * 4 * 2 / math.sqrt(i))
     assert bool((err <= tol).all()), f"{(err / tol).max().item():.3g} of the tolerance"
     if dtype != torch.float32:
         return
     # with an fp32 out every sum is in fp32, and such moves are rare: two fp32 sums of one value differ by some 2^-22 of it, its borders lie 2^-3 apart, so one
     # of 2^19 / (4 sizes of safety) values moves; every other row lies within the roundings alone
-    tight = expert_tolerance(want, mag, k, dtype, 0.0)
+    tight = expert_tolerance(want, mag, i, dtype, 0.0)
     moved = int((err > tight).any(-1).sum())
     assert moved <= 1 + math.ceil(t * k * i * 2.0 ** -17), f"{moved} of {t} rows"
 
@@ -360,9 +372,9 @@ def device(a, gpu):
     return [v.to(gpu) for v in a]
 
 
-def check_experts(out, want, mag, k, i, dtype):
+def check_experts(out, want, mag, i, dtype):
     err = (out.cpu().double() - want).abs()
-    tol = expert_tolerance(want, mag, k, dtype, 0.125 * 4 * 2 / math.sqrt(i))
+    tol = expert_tolerance(want, mag, i, dtype, 0.125 * 4 * 2 / math.sqrt(i))
     assert bool((err <= tol).all()), f"{(err / tol).max().item():.3g} of the tolerance"
 
 
@@ -390,7 +402,7 @@ def test_experts_accumulate_strided_and_on_another_stream(gpu, t):
     assert torch.equal(out[:, :4], base[:, :4]) and torch.equal(out[:, 4 + h:], base[:, 4 + h:])
     # the terms are fp16 (x's type), their sum and the residual fp32
     err = (out[:, 4:4 + h].double() - base[:, 4:4 + h].double() - want).abs()
-    tol = expert_tolerance(want, mag, k, torch.float16, 0.125 * 4 * 2 / math.sqrt(i)) + 2.0 ** -23 * out[:, 4:4 + h].abs()
+    tol = expert_tolerance(want, mag, i, torch.float16, 0.125 * 4 * 2 / math.sqrt(i)) + 2.0 ** -23 * out[:, 4:4 + h].abs()
     assert bool((err <= tol).all())
 
 
@@ -405,7 +417,7 @@ def test_experts_all_tokens_to_one_expert_and_twice(gpu, t, dtype):
     ids[1::2, 1] = -7
     want, mag = experts64(x, ids, weights, *w)
     out = K.moe_experts(*device((x, ids, weights, *w), gpu))
-    check_experts(out, want, mag, k, i, dtype)
+    check_experts(out, want, mag, i, dtype)
 
 
 @pytest.mark.parametrize("t", [3, 90])
@@ -438,7 +450,7 @@ def test_experts_nan_and_infinity_stay_in_their_token(gpu, t):
     rest = torch.tensor([r for r in range(t) if r not in (1, 3)])
     assert not bool(bad[rest].any())
     want, mag = experts64(x[rest], ids[rest], weights[rest], *w)
-    check_experts(out[rest], want, mag, k, i, torch.float16)
+    check_experts(out[rest], want, mag, i, torch.float16)
 
 
 def test_experts_same_inputs_same_bits(gpu):

@@ -51,8 +51,7 @@ def test_block_matches_definition(gpu, rows, shared):
     logits = torch.nn.functional.linear(h, w.gate)
     weights, ids = route64(logits.cpu(), TOP_K, shared_expert=shared)
     want, mag = experts64(h.cpu(), ids, weights.float(), w.w13.cpu(), w.s13.cpu(), w.w2.cpu(), w.s2.cpu())
-    slots = TOP_K + int(shared)
-    tol = expert_tolerance(want, mag, slots, torch.float16, 0.125 * 4 * 2 / INTER ** 0.5) + 2.0 ** -23 * got.abs()
+    tol = expert_tolerance(want, mag, INTER, torch.float16, 0.125 * 4 * 2 / INTER ** 0.5) + 2.0 ** -23 * got.abs()
     assert bool(((got - x.double() - want).abs() <= tol).all())
 
 
