@@ -1,10 +1,14 @@
 // The mixture-of-experts block that runs between the attention layers
 // (qwen36_chat_batch.py:127-178 `batched_moe_step`, qwen36_router.py:96 `route`).
 //
-//   moe_route_kernel    router logits -> each token's experts and weights
-//   moe_plan_kernel     (token, slot) pairs sorted by expert, cut into tiles
-//   x8_tile_kernel      an expert's gate and up rows with SwiGLU, its down rows
-//   moe_combine_kernel  the sum over a token's slots
+//   moe_route_rows_kernel,   router logits -> each token's experts and weights
+//   moe_route_kernel
+//   moe_prepare_kernel,      x to e4m3; (token, slot) pairs sorted by expert and
+//   moe_place_kernel         cut into tiles
+//   x8_tile_kernel           an expert's gate and up rows with SwiGLU, its down rows
+//   moe_combine_kernel       the sum over a token's slots
+//   moe_up_pairs_kernel,     the same for a few tokens, each pair by itself
+//   moe_down_pairs_kernel
 //
 //     (g | u) = W13[e] Q(x_t)      Q: e4m3, a power-of-two scale per 128 values
 //     y_t     = sum_j w[t, j] W2[e_j] Q(SiLU(g) u)
@@ -523,21 +527,22 @@ __device__ __forceinline__ void plan_count(const PlanArgs& a, int block, PlanSha
   __syncthreads();
 }
 
-// Running sums of the experts' pairs and tiles (thread t: experts 4 t .. 4 t +
-// 3), this workgroup's first position of each expert, and its pairs' places.
+// Running sums of the experts' pairs and tiles (thread t: experts per t .. per t
+// + per - 1), this workgroup's first position of each expert, and its pairs' places.
 // Which of an expert's positions a pair gets does not change its results.
 __device__ __forceinline__ void plan_place(const PlanArgs& a, int block, PlanShared& s, const int (&e)[kPlanPer]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (a.experts + 255) / 256;
   int total[4], before[4], sum = 0, tiles = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int x = 4 * tid + j;
+    const int x = per * tid + j;
     total[j] = before[j] = 0;
-    if (x < a.experts) {
+    if (j < per && x < a.experts) {
       if (a.blocks == 1) {
         total[j] = s.count[x];
       } else {
-#pragma unroll 8
+#pragma unroll 16
         for (int b = 0; b < a.blocks; ++b) {
           const int c = a.counts[b * a.experts + x];
           before[j] += b < block ? c : 0;
@@ -571,8 +576,8 @@ __device__ __forceinline__ void plan_place(const PlanArgs& a, int block, PlanSha
   if (block == 0 && tid == 255) *a.ntiles = trun + tiles;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int x = 4 * tid + j;
-    if (x < a.experts) {
+    const int x = per * tid + j;
+    if (j < per && x < a.experts) {
       s.count[x] = run + before[j];
       if (block == 0)
         for (int i = 0; i < total[j]; i += a.tile)
@@ -587,7 +592,9 @@ __device__ __forceinline__ void plan_place(const PlanArgs& a, int block, PlanSha
 }
 
 // First launch: workgroups 0 .. blocks - 1 count their pairs' experts (a lone
-// one places them too), the others quantise x.
+// one places them too), the others quantise x.  16384 tokens of 2048 values in
+// bf16, 8 of 256 experts: 20.5 us (102 MB at 5 TB/s), the placing launch 13 (its
+// chain of loads: ids, the other workgroups' counts).
 template <int XT>
 __global__ __launch_bounds__(256) void moe_prepare_kernel(const PlanArgs a, const QuantArgs q) {
   __shared__ PlanShared s;
@@ -797,9 +804,13 @@ struct CombineArgs {
 constexpr int kCombineAhead = 4;  // slots loaded ahead of their sums
 
 // out[t] (+)= the sum of the token's slots in slot order, in fp32; slots of no
-// expert were never written and are left out.
-template <int DT>
+// expert were never written and are left out (loaded with the others, not used).
+// Bound by the slots' way from HBM.  STREAM: past the caches, where the slots
+// outgrow them: 16384 tokens, 8 slots of 2048 values, 604 MB in 98 us (6.2 TB/s),
+// 116 through the caches.
+template <int DT, bool STREAM>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs a) {
+  constexpr int kRaw = DT == RIA_DT_F32 ? 2 : 1;  // 16-byte loads of a slot
   const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int per = a.hidden / 8;
   const int64_t t = u / per;
@@ -809,26 +820,32 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs a) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) s[i] = 0.f;
   for (int j0 = 0; j0 < a.top_k; j0 += kCombineAhead) {
-    float v[kCombineAhead][8];
+    u32x4 raw[kCombineAhead][kRaw];
+    int id[kCombineAhead];
+    uint32_t e[kCombineAhead];
 #pragma unroll
     for (int j = 0; j < kCombineAhead; ++j) {
-      const int e = j0 + j < a.top_k ? a.ids[t * a.id_stride + j0 + j] : -1;
+      const int at = min(j0 + j, a.top_k - 1);
+      const int64_t pair = t * a.top_k + at;
+      id[j] = a.ids[t * a.id_stride + at];
+      if constexpr (DT != RIA_DT_F32) e[j] = a.slot_e[pair * (a.hidden / 64) + c / 64];
+      const u32x4* p = static_cast<const u32x4*>(a.slots) + (pair * a.hidden + c) / 8 * kRaw;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = 0.f;
-      if (e >= 0 && e < a.experts) {
-        const int64_t pair = t * a.top_k + j0 + j;
-        load_act8<DT>(a.slots, pair * a.hidden + c, v[j]);
-        if constexpr (DT != RIA_DT_F32) {
-          const float scale = x8_scale(a.slot_e[pair * (a.hidden / 64) + c / 64]);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[j][i] *= scale;
-        }
-      }
+      for (int i = 0; i < kRaw; ++i) raw[j][i] = STREAM ? __builtin_nontemporal_load(p + i) : p[i];
     }
 #pragma unroll
-    for (int j = 0; j < kCombineAhead; ++j)
+    for (int j = 0; j < kCombineAhead; ++j) {
+      const bool on = j0 + j < a.top_k && id[j] >= 0 && id[j] < a.experts;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = add_rn(s[i], v[j][i]);
+      for (int i = 0; i < 8; ++i) {
+        float v;
+        if constexpr (DT == RIA_DT_F32)
+          v = __uint_as_float(raw[j][i / 4][i % 4]);
+        else
+          v = f16_bits_to_f32(static_cast<uint16_t>(raw[j][0][i / 2] >> (16 * (i % 2)))) * x8_scale(e[j]);
+        s[i] = add_rn(s[i], on ? v : 0.f);
+      }
+    }
   }
   X8Args o{};
   o.y = a.out;
@@ -1091,13 +1108,15 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
     hipLaunchKernelGGL((moe_prepare_kernel<RIA_DT_F32>), pgrid, dim3(256), 0, st, plan, quant);
   if (plan.blocks > 1) hipLaunchKernelGGL(moe_place_kernel, dim3(plan.blocks), dim3(256), 0, st, plan);
   launch_moe_tiles(*d, l, most, tile, st);
-  const CombineArgs c{at(l.slots), static_cast<const uint8_t*>(at(l.slot_e)), d->ids, d->ids_row_stride, d->tokens, d->top_k, d->experts, d->hidden, d->out,
-                      d->out_dtype, d->out_row_stride, d->accumulate != 0,
+  const CombineArgs c{at(l.slots), static_cast<const uint8_t*>(at(l.slot_e)), d->ids, d->ids_row_stride, d->tokens,
+                      d->top_k, d->experts, d->hidden, d->out, d->out_dtype, d->out_row_stride, d->accumulate != 0,
                       reinterpret_cast<uintptr_t>(d->out) % 16 == 0 && d->out_row_stride % 8 == 0};
   const dim3 grid(static_cast<unsigned>(((int64_t)d->tokens * (d->hidden / 8) + 255) / 256));
   if (d->x_dtype == RIA_DT_F32)
-    hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F32>), grid, dim3(256), 0, st, c);
+    hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F32, false>), grid, dim3(256), 0, st, c);
+  else if (tile == 256)
+    hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F16, true>), grid, dim3(256), 0, st, c);
   else
-    hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F16>), grid, dim3(256), 0, st, c);
+    hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F16, false>), grid, dim3(256), 0, st, c);
   return check_launch(who);
 }

@@ -298,6 +298,13 @@ __device__ __forceinline__ int x8_order(int b, int total) {
 // step stages one block of K, 128 bytes a row, in LDS by direct copies, chunk
 // c of row r at chunk c ^ ((r >> 1) & 7), so that the 16 lanes of a read's
 // phase meet all 64 banks; the next step's copies run beside the products.
+//
+// Large tiles (4, 2, 2, 4: 256 x 256, one workgroup a CU) are bound by the matrix
+// cores at the clock they allow, beside 64 KB of LDS copies, 128 KB of LDS reads
+// and the scaling's FMAs a step: some 2 us a step, 6 outside the steps.  16384 x
+// 8192 x 2048 to fp16 in 300 us, 1.83 PFLOP/s; 128 x 256 tiles with one LDS
+// buffer, two workgroups a CU: 330 (and the experts' products the same as now).
+// Small tiles (32 or 64 rows) are bound by the weights' way from HBM.
 template <int MODE, int WF, int WT, int NF, int NT, bool WIDE, bool STREAM = false>
 __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
   constexpr int NW = NF * NT;
@@ -478,8 +485,19 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
         for (int i = 0; i < 16; ++i) {
           const float v = x8_swiglu(acc[f][t][i], acc[HF + f][t][i]);
           acc[f][t][i] = v;
-          m = fmaxf(m, finite_abs(v));
+          m = fmaxf(m, fabsf(v));
         }
+      if (__ballot(m == __builtin_inff())) {  // infinities set no scale, and are NaN in e4m3
+        m = 0.f;
+#pragma unroll
+        for (int f = 0; f < HF; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float v = acc[f][t][i];
+            m = fmaxf(m, finite_abs(v));
+            acc[f][t][i] = x8_value(v, 1.f);
+          }
+      }
       const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
       m = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
       if (half == 0) top[wf * BM + (wt * WT + t) * 32 + l32] = m;
@@ -501,7 +519,7 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
         for (int q = 0; q < 4; ++q) {
           float v[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] = x8_value(acc[f][t][4 * q + i], inv);
+          for (int i = 0; i < 4; ++i) v[i] = acc[f][t][4 * q + i] * inv;
           const int o = (wf * HF + f) * 32 + 8 * q + 4 * half;  // byte of the row
           *reinterpret_cast<uint32_t*>(stage + r * 128 + (((o >> 4) ^ (r & 7)) << 4) + (o & 15)) =
               pack_x8(v[0], v[1], v[2], v[3]);
@@ -527,22 +545,31 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
       }
 #pragma unroll
       for (int f0 = 0; f0 < WF; f0 += 2) {
-        float scale = pw;
+        float scale = 1.f;
         if constexpr (MODE == kX8Down) {
+          float top = 0.f;
+#pragma unroll
+          for (int f = 0; f < 2; ++f)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float v = pw * acc[f0 + f][t][i];
+              acc[f0 + f][t][i] = v;
+              top = fmaxf(top, fabsf(v));
+            }
           if (a.y_dtype != RIA_DT_F32) {
-            float top = 0.f;
+            if (__ballot(top == __builtin_inff())) {  // infinities set no scale
+              top = 0.f;
 #pragma unroll
-            for (int f = 0; f < 2; ++f)
+              for (int f = 0; f < 2; ++f)
 #pragma unroll
-              for (int i = 0; i < 16; ++i) top = fmaxf(top, finite_abs(pw * acc[f0 + f][t][i]));
+                for (int i = 0; i < 16; ++i) top = fmaxf(top, finite_abs(acc[f0 + f][t][i]));
+            }
             const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             const uint32_t e = term_scale_exp(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])));
             scale = x8_inverse(e);
             const int rr = (wt * WT + t) * 32 + l32, g = (n0 + (wf * WF + f0) * 32) / 64;
             if (half == 0 && rr < rows && g < a.ye_stride)
               a.ye[(int64_t)a.order[first + rr] * a.ye_stride + g] = static_cast<uint8_t>(e);
-          } else {
-            scale = 1.f;
           }
         }
 #pragma unroll
@@ -551,8 +578,7 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
           for (int q = 0; q < 4; ++q) {
             f32x4 v;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              v[i] = MODE == kX8Down ? pw * acc[f0 + f][t][4 * q + i] * scale : acc[f0 + f][t][4 * q + i];
+            for (int i = 0; i < 4; ++i) v[i] = MODE == kX8Down ? acc[f0 + f][t][4 * q + i] * scale : acc[f0 + f][t][4 * q + i];
             *reinterpret_cast<f32x4*>(st + l32 * kPitch + f * 32 + 8 * q + 4 * half) = v;
           }
 #pragma unroll
