@@ -154,6 +154,14 @@ __device__ __forceinline__ void route_shared(const RouteArgs& a, int64_t t) {
   a.ids[t * a.id_stride + a.top_k] = l == -__builtin_inff() ? -1 : a.experts;
 }
 
+// A value of lane 7 - l of each 8.
+__device__ __forceinline__ uint32_t half_mirror(uint32_t u) {
+  return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(u), 0x141, 0xf, 0xf, true));
+}
+__device__ __forceinline__ uint64_t half_mirror(uint64_t u) {
+  return static_cast<uint64_t>(half_mirror(static_cast<uint32_t>(u >> 32))) << 32 | half_mirror(static_cast<uint32_t>(u));
+}
+
 // Largest over each row of 16 lanes.
 template <typename T>
 __device__ __forceinline__ T row_max(T v) {
@@ -161,98 +169,6 @@ __device__ __forceinline__ T row_max(T v) {
   v = max(v, lane_xor<4>(v));
   v = max(v, lane_xor<2>(v));
   return max(v, lane_xor<1>(v));
-}
-
-// Scores that grow with the logits, no groups, up to 256 experts and 16 of them
-// chosen: four tokens a wave, 16 lanes each, lane l holding experts V l .. V l +
-// V - 1 of its token.  A key is a logit's order with the expert's complement
-// below it (32 bits where the logits have 16, else 64), so no two are equal and
-// the lowest index wins ties by itself.  Each lane sorts its keys (an odd-even
-// merge network: no branches), and the token's best is then the largest of 16
-// heads, top_k times.  Against one wave per token and the best of all keys each
-// time, which waits on its lane exchanges: 16384 tokens, 8 of 256, 15.1 us in
-// the kernel, now 6.8 (instructions; the logits' 8.4 MB take 1.6).
-template <int XT, int V, int KM>
-__global__ __launch_bounds__(64 * kRouteWaves) void moe_route_rows_kernel(const RouteArgs a) {
-  constexpr bool kNarrow = XT != RIA_DT_F32;
-  constexpr int kLow = XT == RIA_DT_BF16 ? 16 : XT == RIA_DT_F16 ? 13 : 32;  // bits of a key below the logit's
-  constexpr int kList = KM < V ? KM : V;                                      // a lane's keys that can be taken
-  using Key = std::conditional_t<kNarrow, uint32_t, uint64_t>;
-  constexpr Key kMask = (Key(1) << kLow) - 1;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
-  const int64_t row = ((int64_t)blockIdx.x * kRouteWaves + wave) * 4 + (lane >> 4);
-  const int64_t t = min(row, (int64_t)a.tokens - 1);  // rows past the last repeat it, and store nothing
-  const int e = a.experts;
-  const float ninf = -__builtin_inff();
-  float x[V];
-  load_logits<XT, V>(a, t, l16 * V, x);
-  auto top_bits = [](uint32_t o) { return kNarrow ? static_cast<Key>(o >> kLow % 32 << kLow % 32) : static_cast<Key>(o) << kLow % 64; };
-  Key key[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int i = l16 * V + v;
-    const Key k = top_bits(order_key(x[v])) | (kMask - static_cast<Key>(i));
-    key[v] = i < e ? k : 0;
-  }
-#pragma unroll
-  for (int p = 1; p < V; p *= 2)
-#pragma unroll
-    for (int k = p; k >= 1; k /= 2)
-#pragma unroll
-      for (int j = k % p; j + k < V; j += 2 * k)
-#pragma unroll
-        for (int i = 0; i < k; ++i)
-          if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
-            const Key lo = min(key[i + j], key[i + j + k]);
-            key[i + j] = max(key[i + j], key[i + j + k]);
-            key[i + j + k] = lo;
-          }
-  Key mine = 0, first = 0;
-  for (int j = 0; j < a.top_k; ++j) {
-    const Key best = row_max(key[0]);
-    const bool taken = key[0] == best;
-#pragma unroll
-    for (int v = 0; v + 1 < kList; ++v) {  // (values, not elements, to choose from: no index of the lane's own)
-      const Key here = key[v], next = key[v + 1];
-      key[v] = taken ? next : here;
-    }
-    key[kList - 1] = taken ? 0 : key[kList - 1];
-    if (j == 0) first = best;
-    if (l16 == j) mine = best;
-  }
-  auto value = [&](Key k) {  // the logit of a key
-    uint32_t o = static_cast<uint32_t>(kNarrow ? k >> kLow % 32 << kLow % 32 : k >> kLow % 64);
-    if (kNarrow && !(o >> 31)) o |= static_cast<uint32_t>(kMask);  // a negative one's zeros are ones in its order
-    return key_value(o);
-  };
-  const Key none = top_bits(order_key(ninf)) | kMask;
-  const bool chosen = mine > none;
-  const float my_x = chosen ? value(mine) : ninf;
-  const float m0 = first > none ? value(first) : 0.f;  // the largest logit, NaN if there is one
-  float w = 0.f;
-  if (a.renorm) {
-    if (chosen) w = a.sigmoid ? sigmoid_from(my_x, m0) : exp_diff(my_x, m0);
-    float sum = add_xor<8>(w);
-    sum = add_rn(sum, __uint_as_float(lane_xor<4>(__float_as_uint(sum))));
-    sum = add_xor<1>(add_xor<2>(sum));
-    if (sum != 0.f) w = w / sum;
-  } else if (a.sigmoid) {
-    if (chosen) w = 1.f / (1.f + expf(-my_x));
-  } else {
-    float sum = 0.f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) sum += exp_diff(x[v], m0);
-    sum = add_xor<8>(sum);
-    sum = add_rn(sum, __uint_as_float(lane_xor<4>(__float_as_uint(sum))));
-    sum = add_xor<1>(add_xor<2>(sum));
-    if (chosen) w = exp_diff(my_x, m0) / sum;
-  }
-  if (row >= a.tokens) return;
-  if (l16 < a.top_k) {
-    a.weights[t * a.w_stride + l16] = w * a.scale;
-    a.ids[t * a.id_stride + l16] = chosen ? static_cast<int>(kMask - (mine & kMask)) : -1;
-  }
-  if (a.shared && l16 == 15) route_shared<XT>(a, t);
 }
 
 // Whether two fp32 choices lie too near for their order to be sure: scores are
@@ -366,14 +282,243 @@ __device__ __forceinline__ bool route_select(const RouteArgs& a, int lane, Key (
   return sure;
 }
 
-// One wave per token: groups, biases, many experts.  SCORED: choices are scores
-// (with a bias, or ranked by sums), which are compared in fp32 first; where
-// their order is not sure, which takes choices within some 2^-18 of each other,
-// the token is chosen again with scores in 64 bits, so that the ids are the
-// formula's.  Otherwise scores grow with the logits, which are compared
-// themselves.  256 experts in 8 groups with a bias: 16384 tokens 34 us, 41 in 64
-// bits throughout (65536: 101 and 145).  At 4099 tokens both take 16: some
-// tokens of a batch are chosen again, and 4 us of that show at the end.
+// The same from scores in 64 bits, where the fp32 ones did not decide.  top: the
+// softmax's largest logit.
+template <int V>
+__device__ void route_select_wide(const RouteArgs& a, int lane, const float (&x)[V], float top, uint64_t* s, int& my_id,
+                                  float& my_x) {
+  const float ninf = -__builtin_inff();
+  double total = 1.0;
+  if (!a.sigmoid) {
+    double sum = 0.0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum += exp(static_cast<double>(x[v]) - static_cast<double>(top));
+    total = wave_sum64(sum);
+    if (total == 0.0) total = 1.0;
+  }
+  uint64_t key[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = lane * V + v;
+    const double l = x[v];
+    const double p = a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - static_cast<double>(top)) / total;
+    const double c = x[v] == ninf ? static_cast<double>(ninf) : p + (a.bias ? static_cast<double>(a.bias[min(i, a.experts - 1)]) : 0.0);
+    key[v] = i < a.experts ? order_key(c) : 0;
+  }
+  __builtin_amdgcn_wave_barrier();
+  route_select<uint64_t, V, false>(a, lane, key, x, s, my_id, my_x);
+}
+
+// An fp32 score's choice.  top, total: the softmax's largest logit and sum.
+__device__ __forceinline__ float route_choice(const RouteArgs& a, float x, float bias, float top, float total) {
+  const float p = a.sigmoid ? 1.f / (1.f + expf(-x)) : exp_diff(x, top) / total;
+  return x == -__builtin_inff() ? x : p + bias;
+}
+
+// Whether the token's groups are whole lanes of V experts each, a power of two
+// of them.
+static bool route_groups_fit(const RouteArgs& a, int v) {
+  const int per = a.experts / a.groups, lanes = per / v;
+  return a.groups == 1 || (per % v == 0 && (lanes & (lanes - 1)) == 0);
+}
+
+// Up to 256 experts and 16 of them chosen: four tokens a wave, 16 lanes each,
+// lane l holding experts V l .. V l + V - 1 of its token.  A key is a choice's
+// order with the expert's complement below it (32 bits where choices are 16-bit
+// logits, else 64), so no two are equal and the lowest index wins ties by
+// itself.  Each lane sorts its keys (an odd-even merge network: no branches),
+// and the token's best is then the largest of 16 heads, top_k times.  SCORED:
+// choices are scores (with a bias, or ranked by sums), compared in fp32; a token
+// whose order is not sure, which takes choices within some 2^-18 of each other,
+// is chosen again by the whole wave with scores in 64 bits, so that the ids are
+// the formula's.
+//
+// Bound by instructions and, at few tokens, by their latencies.  Against one
+// wave per token and the best of all keys each time, which waits on its lane
+// exchanges: 16384 tokens, 8 of 256, 15.1 us in the kernel, now 6.8 (the logits'
+// 8.4 MB take 1.6).
+template <int XT, int V, int KM, bool SCORED>
+__global__ __launch_bounds__(64 * kRouteWaves) void moe_route_rows_kernel(const RouteArgs a) {
+  constexpr bool kNarrow = XT != RIA_DT_F32 && !SCORED;
+  constexpr int kLow = !kNarrow ? 32 : XT == RIA_DT_BF16 ? 16 : 13;  // bits of a key below the choice's
+  constexpr int kList = KM + (SCORED ? 1 : 0) < V ? KM + (SCORED ? 1 : 0) : V;  // a lane's keys that are looked at
+  constexpr int kWide = V / 4;                                       // experts a lane takes with a wave to a token
+  using Key = std::conditional_t<kNarrow, uint32_t, uint64_t>;
+  constexpr Key kMask = (Key(1) << kLow) - 1;
+  __shared__ float logits_s[SCORED ? kRouteWaves : 1][SCORED ? 4 * 16 * V : 1];
+  __shared__ uint64_t wide_s[SCORED ? kRouteWaves : 1][SCORED ? 64 * kWide : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15;
+  const int64_t row = ((int64_t)blockIdx.x * kRouteWaves + wave) * 4 + (lane >> 4);
+  const int64_t t = min(row, (int64_t)a.tokens - 1);  // rows past the last repeat it, and store nothing
+  const int e = a.experts;
+  const float ninf = -__builtin_inff();
+  auto row_sum = [](float v) {
+    v = add_xor<8>(v);
+    v = add_rn(v, __uint_as_float(lane_xor<4>(__float_as_uint(v))));
+    return add_xor<1>(add_xor<2>(v));
+  };
+  float x[V];
+  load_logits<XT, V>(a, t, l16 * V, x);
+  auto top_bits = [](uint32_t o) { return kNarrow ? static_cast<Key>(o >> kLow % 32 << kLow % 32) : static_cast<Key>(o) << kLow % 64; };
+  auto order_of = [](Key k) {  // the order key of a key's choice
+    uint32_t o = static_cast<uint32_t>(kNarrow ? k >> kLow % 32 << kLow % 32 : k >> kLow % 64);
+    if (kNarrow && !(o >> 31)) o |= static_cast<uint32_t>(kMask);  // a negative one's zeros are ones in its order
+    return o;
+  };
+  float top = 0.f, total = 1.f;  // of the softmax: its largest logit (NaN if there is one) and its sum
+  Key key[V];
+  if constexpr (SCORED) {
+    float bias[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) bias[v] = a.bias ? a.bias[min(l16 * V + v, e - 1)] : 0.f;
+#pragma unroll
+    for (int v = 0; v < V; v += 4)
+      *reinterpret_cast<f32x4*>(&logits_s[wave][lane * V + v]) = f32x4{x[v], x[v + 1], x[v + 2], x[v + 3]};
+    if (!a.sigmoid) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) m = max(m, order_key(x[v]));
+      top = key_value(row_max(m));
+      if (top == ninf) top = 0.f;
+      float s = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) s += exp_diff(x[v], top);
+      total = row_sum(s);
+      if (total == 0.f) total = 1.f;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = l16 * V + v;
+      const Key k = top_bits(order_key(route_choice(a, x[v], bias[v], top, total))) | (kMask - static_cast<Key>(i));
+      key[v] = i < e ? k : 0;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = l16 * V + v;
+      const Key k = top_bits(order_key(x[v])) | (kMask - static_cast<Key>(i));
+      key[v] = i < e ? k : 0;
+    }
+  }
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < V; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const Key lo = min(key[i + j], key[i + j + k]);
+            key[i + j] = max(key[i + j], key[i + j + k]);
+            key[i + j + k] = lo;
+          }
+  const uint32_t none32 = order_key(ninf);
+  bool sure = true;
+  if (a.groups > 1) {  // a group is 1, 2, 4 or 8 whole lanes
+    const int lanes = e / a.groups / V, g = l16 / lanes;
+    Key b0 = key[0], b1 = key[1];  // the group's best two
+    auto meet = [&](Key o0, Key o1) {
+      b1 = max(min(b0, o0), max(b1, o1));
+      b0 = max(b0, o0);
+    };
+    if (lanes >= 2) meet(lane_xor<1>(b0), lane_xor<1>(b1));
+    if (lanes >= 4) meet(lane_xor<2>(b0), lane_xor<2>(b1));
+    if (lanes >= 8) meet(half_mirror(b0), half_mirror(b1));
+    uint32_t rank = SCORED && a.top2 ? order_key(key_sum(order_of(b0), order_of(b1))) : order_of(b0);
+    rank = g < a.groups ? rank : 0;
+    int better = 0;  // groups that come before this one
+    for (int j = 0; j < a.groups; ++j) {
+      const uint32_t o = static_cast<uint32_t>(__shfl(static_cast<int>(rank), (lane & 48) + j * lanes));
+      better += o > rank || (o == rank && j < g);
+    }
+    const bool in = g < a.groups && better < a.top_groups;
+    if constexpr (SCORED) {
+      const uint32_t best_out = row_max(in ? 0u : rank), worst_in = ~row_max(in ? ~rank : 0u);
+      if (best_out > none32 && unsure(worst_in, best_out)) sure = false;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = in ? key[v] : 0;
+  }
+  Key mine = 0, first = 0, last = 0;
+  for (int j = 0; j < a.top_k + (SCORED ? 1 : 0); ++j) {
+    const Key best = row_max(key[0]);
+    if constexpr (SCORED) {
+      if (j > 0 && order_of(best) > none32 && unsure(order_of(last), order_of(best))) sure = false;
+      if (j == a.top_k) break;  // looked at only
+      last = best;
+    }
+    const bool taken = key[0] == best;
+#pragma unroll
+    for (int v = 0; v + 1 < kList; ++v) {  // (values, not elements, to choose from: no index of the lane's own)
+      const Key here = key[v], next = key[v + 1];
+      key[v] = taken ? next : here;
+    }
+    key[kList - 1] = taken ? 0 : key[kList - 1];
+    if (j == 0) first = best;
+    if (l16 == j) mine = best;
+  }
+  bool chosen = order_of(mine) > none32;
+  int my_id = chosen ? static_cast<int>(kMask - (mine & kMask)) : -1;
+  float my_x = ninf, m0 = 0.f;  // this lane's logit; the largest of the chosen ones, NaN if there is one
+  if constexpr (SCORED) {
+    __builtin_amdgcn_wave_barrier();
+    if (chosen) my_x = logits_s[wave][(lane & 48) * V + my_id];
+    uint64_t again = __ballot(!sure);
+    while (again) {  // (the wave's: a token at a time)
+      const int from = __builtin_ctzll(again) & 48;
+      again &= ~(uint64_t(0xffff) << from);
+      float wx[kWide];
+#pragma unroll
+      for (int v = 0; v < kWide; ++v) wx[v] = logits_s[wave][from * V + lane * kWide + v];
+      const float its_top = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(top), from));
+      int id;
+      float idx;
+      route_select_wide<kWide>(a, lane, wx, its_top, wide_s[wave], id, idx);
+      id = __shfl(id, l16);
+      idx = __shfl(idx, l16);
+      if ((lane & 48) == from) {
+        my_id = id;
+        my_x = idx;
+      }
+    }
+    chosen = my_id >= 0;
+    const uint32_t m = row_max(chosen ? order_key(my_x) : 0u);
+    if (m) m0 = key_value(m);
+  } else {
+    if (chosen) my_x = key_value(order_of(mine));
+    if (order_of(first) > none32) m0 = key_value(order_of(first));
+  }
+  float w = 0.f;
+  if (a.renorm) {  // about the largest chosen logit: the weights hold where every score underflows
+    if (chosen) w = a.sigmoid ? sigmoid_from(my_x, m0) : exp_diff(my_x, m0);
+    if (SCORED && !a.sigmoid && total != total) w = __builtin_nanf("");  // a NaN logit that was not chosen
+    const float sum = row_sum(w);
+    if (sum != 0.f) w = w / sum;
+  } else if (a.sigmoid) {
+    if (chosen) w = 1.f / (1.f + expf(-my_x));
+  } else {
+    if constexpr (!SCORED) {
+      top = m0;  // (the largest logit's group is always open)
+      float s = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) s += exp_diff(x[v], top);
+      total = row_sum(s);
+    }
+    if (chosen) w = exp_diff(my_x, top) / total;
+  }
+  if (row >= a.tokens) return;
+  if (l16 < a.top_k) {
+    a.weights[t * a.w_stride + l16] = w * a.scale;
+    a.ids[t * a.id_stride + l16] = my_id;
+  }
+  if (a.shared && l16 == 15) route_shared<XT>(a, t);
+}
+
+// One wave per token: scores of few tokens, many experts, groups of no whole
+// lanes.  SCORED as above: 4099 tokens, 256 experts in 8 groups with a bias, 16 us
+// both with the guarded fp32 scores and in 64 bits throughout (some tokens of a
+// batch are chosen again, and 4 us of that show at the end); 16384 tokens 34 and 41.
 template <int XT, int V, bool SCORED>
 __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const RouteArgs a) {
   __shared__ uint64_t group_s[kRouteWaves][64 * V];
@@ -407,30 +552,11 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
     uint32_t key[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float p = a.sigmoid ? 1.f / (1.f + expf(-x[v])) : exp_diff(x[v], top) / total;
-      const float c = x[v] == ninf ? ninf : p + bias[v];
-      key[v] = lane * V + v < e ? order_key(c) : 0;
+      const uint32_t k = order_key(route_choice(a, x[v], bias[v], top, total));
+      key[v] = lane * V + v < e ? k : 0;
     }
-    if (!route_select<uint32_t, V, true>(a, lane, key, x, reinterpret_cast<uint32_t*>(group_s[wave]), my_id, my_x)) {
-      double wide_total = 1.0;
-      if (!a.sigmoid) {
-        double s = 0.0;
-#pragma unroll
-        for (int v = 0; v < V; ++v) s += exp(static_cast<double>(x[v]) - static_cast<double>(top));
-        wide_total = wave_sum64(s);
-        if (wide_total == 0.0) wide_total = 1.0;
-      }
-      uint64_t wide[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const double l = x[v];
-        const double p = a.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - static_cast<double>(top)) / wide_total;
-        const double c = x[v] == ninf ? static_cast<double>(ninf) : p + static_cast<double>(bias[v]);
-        wide[v] = lane * V + v < e ? order_key(c) : 0;
-      }
-      __builtin_amdgcn_wave_barrier();
-      route_select<uint64_t, V, false>(a, lane, wide, x, group_s[wave], my_id, my_x);
-    }
+    if (!route_select<uint32_t, V, true>(a, lane, key, x, reinterpret_cast<uint32_t*>(group_s[wave]), my_id, my_x))
+      route_select_wide<V>(a, lane, x, top, group_s[wave], my_id, my_x);
   } else {
     uint32_t key[V];
 #pragma unroll
@@ -460,19 +586,28 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
   if (a.shared && lane == 63) route_shared<XT>(a, t);
 }
 
+// Scores of fewer tokens are chosen by a wave each: its chain of instructions is
+// shorter, and the card is not full.  256 experts, a wave for four tokens / for
+// one: with 8 groups and a bias 4099 tokens 16.7 / 15.9 us, 12000 tokens 23.0 /
+// 27.2, 65536 tokens 60.6 / 102; with a bias alone 13.5 / 11.5, 19.4 / 19.1, 52.4 /
+// 70; a softmax with a bias 15.2 / 12.5, 22.0 / 21.0, 62 / 78.  (Groups ranked by
+// their largest logit: 4099 tokens 7.3 / 9.3, 65536 tokens 33 / 72.)
+constexpr int kRouteRowsTokens = 12288;
+
 template <int XT, bool SCORED>
 static void launch_route(const RouteArgs& a, hipStream_t st) {
-  if (!SCORED && a.groups == 1 && a.experts <= 256 && a.top_k <= 16) {
+  const bool few = a.top_k <= 8;
+  const int per_lane = a.experts <= 64 ? 4 : a.experts <= 128 && few ? 8 : 16;
+  if (a.experts <= 256 && a.top_k <= 16 && route_groups_fit(a, per_lane) && (!SCORED || a.tokens >= kRouteRowsTokens)) {
     const dim3 grid((a.tokens + 4 * kRouteWaves - 1) / (4 * kRouteWaves)), block(64 * kRouteWaves);
-    const bool few = a.top_k <= 8;
-    if (a.experts <= 64)
-      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 4, 16>), grid, block, 0, st, a);
-    else if (a.experts <= 128 && few)
-      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 8, 8>), grid, block, 0, st, a);
+    if (per_lane == 4)
+      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 4, 16, SCORED>), grid, block, 0, st, a);
+    else if (per_lane == 8)
+      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 8, 8, SCORED>), grid, block, 0, st, a);
     else if (few)
-      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 16, 8>), grid, block, 0, st, a);
+      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 16, 8, SCORED>), grid, block, 0, st, a);
     else
-      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 16, 16>), grid, block, 0, st, a);
+      hipLaunchKernelGGL((moe_route_rows_kernel<XT, 16, 16, SCORED>), grid, block, 0, st, a);
     return;
   }
   const dim3 grid((a.tokens + kRouteWaves - 1) / kRouteWaves), block(64 * kRouteWaves);

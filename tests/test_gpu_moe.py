@@ -235,13 +235,26 @@ ROUTES = [
     dict(t=30, e=512, k=16, bias=True, scale=0.5, renormalize=False),
     dict(t=9, e=1000, k=32, num_groups=4, top_groups=2, bias=True, shared_expert=True),
     dict(t=9, e=1, k=1),
+    # groups of 1, 4 and 8 lanes of a wave that takes four tokens; of no whole lanes, or no power of two of them
+    dict(t=50, e=256, k=16, bias=True, num_groups=16, top_groups=3),
+    dict(t=50, e=128, k=6, num_groups=4, top_groups=2, group_score="top2", renormalize=False),
+    dict(t=50, e=256, k=8, scoring="sigmoid", num_groups=2, top_groups=1, group_score="max", renormalize=False),
+    dict(t=50, e=48, k=4, bias=True, num_groups=3, top_groups=2, group_score="max", shared_expert=True),
+    dict(t=50, e=64, k=5, scoring="sigmoid", bias=True, num_groups=2, top_groups=2, scale=3.0),
+    dict(t=50, e=256, k=8, bias=True, num_groups=64, top_groups=9),
+    dict(t=50, e=96, k=3, bias=True, num_groups=2, top_groups=1),
+    dict(t=50, e=256, k=8, scoring="softmax", num_groups=2, top_groups=1, group_score="max", renormalize=False),
 ]
+
+
+MANY = 12288 + 3  # tokens past which a wave takes four of them where scores are compared
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("case", ROUTES, ids=lambda c: f"t{c['t']}_e{c['e']}_k{c['k']}")
 @pytest.mark.parametrize("masked", [False, True])
-def test_route_matches_definition(gpu, case, dtype, masked):
+@pytest.mark.parametrize("many", [False, True])
+def test_route_matches_definition(gpu, case, dtype, masked, many):
     c = dict(case)
     t, e, k = c.pop("t"), c.pop("e"), c.pop("k")
     announce(f"moe_route: {t} tokens, {k} of {e} {dtype} {c} masked {masked}")
@@ -253,6 +266,8 @@ def test_route_matches_definition(gpu, case, dtype, masked):
     if c.pop("bias", False):
         c["bias"] = torch.randn((e,), generator=gen(3)) * 0.2
     want_w, want_i = route64(x, k, **c)
+    if many:  # the same tokens again and again
+        x, want_w, want_i = (v.repeat(MANY // t + 1, 1)[:MANY] for v in (x, want_w, want_i))
     if "bias" in c:
         c["bias"] = c["bias"].to(gpu)
     wide = torch.nn.functional.pad(x, (0, 5)).to(gpu)[:, :cols]
@@ -275,7 +290,8 @@ def test_route_ties_go_to_the_lowest_index(gpu):
     assert i.cpu().tolist() == [[0, 1, 2]]
 
 
-def test_route_near_ties_follow_64_bits(gpu):
+@pytest.mark.parametrize("many", [False, True])
+def test_route_near_ties_follow_64_bits(gpu, many):
     """A bias that brings unlike scores within 1e-9 of each other: fp32 could not order them."""
     announce("moe_route: scores and biases that nearly cancel")
     g = gen(5)
@@ -283,7 +299,27 @@ def test_route_near_ties_follow_64_bits(gpu):
     p = torch.sigmoid(x[0].double())
     bias = (1.0 - p).float()  # token 0: every choice within fp32 roundings of 1
     want_w, want_i = route64(x, 8, scoring="sigmoid", bias=bias)
+    if many:
+        x, want_w, want_i = (v.repeat(MANY // 64 + 1, 1)[:MANY] for v in (x, want_w, want_i))
     w, i = K.moe_route(x.to(gpu), 8, scoring="sigmoid", bias=bias.to(gpu))
+    assert torch.equal(i.cpu(), want_i)
+    torch.testing.assert_close(w.cpu().double(), want_w, rtol=16 * 2.0 ** -24, atol=0)
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("groups", [1, 8])
+def test_route_near_ties_in_one_place(gpu, groups, many):
+    """The chosen experts and the next one, 1e-9 apart, are neighbours; every other token is far from a tie."""
+    announce(f"moe_route: near ties in experts 16 to 31, {groups} groups")
+    x = torch.randn((37, 256), generator=gen(6))
+    p = torch.sigmoid(x[5].double())
+    bias = torch.full((256,), -3.0)
+    bias[16:32] = (1.0 - p[16:32]).float()
+    c = dict(scoring="sigmoid", num_groups=groups, top_groups=max(groups // 2, 1))
+    want_w, want_i = route64(x, 8, bias=bias, **c)
+    if many:
+        x, want_w, want_i = (v.repeat(MANY // 37 + 1, 1)[:MANY] for v in (x, want_w, want_i))
+    w, i = K.moe_route(x.to(gpu), 8, bias=bias.to(gpu), **c)
     assert torch.equal(i.cpu(), want_i)
     torch.testing.assert_close(w.cpu().double(), want_w, rtol=16 * 2.0 ** -24, atol=0)
 
@@ -307,6 +343,26 @@ def test_route_extreme_logits(gpu):
     w, i = K.moe_route(x.to(gpu), 2, scoring="sigmoid")
     assert i[1].tolist() == [15, 14] and i[0].tolist() == [3, 0]
     torch.testing.assert_close(w[0].cpu(), torch.tensor([1.0, math.exp(-10.0)]) / (1 + math.exp(-10.0)), rtol=1e-6, atol=0)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [1, 2])
+def test_route_extreme_logits_of_many_tokens(gpu, scoring, groups):
+    """Tokens with infinities and NaN choose the same experts in a large batch as in a small one."""
+    announce(f"moe_route: infinite and NaN logits, {scoring}, {groups} groups, {MANY} tokens")
+    x = torch.randn((7, 64), generator=gen(8))
+    x[0, 40], x[0, 9] = math.nan, 5.0
+    x[1, 4] = math.inf
+    x[2, 3:] = -math.inf
+    x[3] = math.nan
+    x[4, 7], x[4, 50] = 3e38, -3e38
+    x[5] = -200.0
+    c = dict(scoring=scoring, bias=torch.linspace(0, 0.5, 64).to(gpu), num_groups=groups, top_groups=1)
+    want_w, want_i = K.moe_route(x.to(gpu), 4, **c)
+    w, i = K.moe_route(x.repeat(MANY // 7 + 1, 1)[:MANY].to(gpu), 4, **c)
+    assert torch.equal(i, want_i.repeat(MANY // 7 + 1, 1)[:MANY])
+    # both sum and divide in fp32, in orders of their own
+    torch.testing.assert_close(w, want_w.repeat(MANY // 7 + 1, 1)[:MANY], rtol=32 * 2.0 ** -24, atol=0, equal_nan=True)
 
 
 # ----------------------------------------------------------------------------- experts
