@@ -11,7 +11,7 @@ step of every layer is one launch over the batch, and the projections read
 the checkpoint's FP8 block-scaled weights as stored.  The MoE block (and the
 embedding, final norm and lm_head around the loop) stay the caller's: pass a
 callable ``mlp(model_layer, x) -> x`` to run between layers, as the
-reference does.
+reference does (``moe_block.MoeBlock`` is one).
 
 Per layer (B rows, hidden 2048, the reference's CUDA dtypes):
 
