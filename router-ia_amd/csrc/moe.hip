@@ -634,7 +634,8 @@ struct PlanArgs {
   int blocks;      // planning workgroups: ceil(pairs / kPlanPairs)
   int tile;        // pairs of one expert in a tile
   int32_t* counts; // [blocks, experts] (more than one workgroup)
-  int32_t* order;
+  int32_t* order;  // the pair at each position of the sorted ones
+  int32_t* where;  // the position of each pair of an expert
   X8Tile* tiles;
   int32_t* ntiles;
 };
@@ -664,7 +665,9 @@ __device__ __forceinline__ void plan_count(const PlanArgs& a, int block, PlanSha
 
 // Running sums of the experts' pairs and tiles (thread t: experts per t .. per t
 // + per - 1), this workgroup's first position of each expert, and its pairs' places.
-// Which of an expert's positions a pair gets does not change its results.
+// Which of an expert's positions a pair gets does not change its results.  Terms
+// are kept in the order of the positions, so that a tile's stores are neighbours:
+// 16384 tokens' down rows 362 us, 385 with the terms at their pairs' places.
 __device__ __forceinline__ void plan_place(const PlanArgs& a, int block, PlanShared& s, const int (&e)[kPlanPer]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int per = (a.experts + 255) / 256;
@@ -723,12 +726,16 @@ __device__ __forceinline__ void plan_place(const PlanArgs& a, int block, PlanSha
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kPlanPer; ++i)
-    if (e[i] >= 0) a.order[atomicAdd(&s.count[e[i]], 1)] = block * kPlanPairs + i * 256 + tid;
+    if (e[i] >= 0) {
+      const int pair = block * kPlanPairs + i * 256 + tid, at = atomicAdd(&s.count[e[i]], 1);
+      a.order[at] = pair;
+      a.where[pair] = at;
+    }
 }
 
 // First launch: workgroups 0 .. blocks - 1 count their pairs' experts (a lone
 // one places them too), the others quantise x.  16384 tokens of 2048 values in
-// bf16, 8 of 256 experts: 20.5 us (102 MB at 5 TB/s), the placing launch 13 (its
+// bf16, 8 of 256 experts: 20.5 us (102 MB at 5 TB/s), the placing launch 16 (its
 // chain of loads: ids, the other workgroups' counts).
 template <int XT>
 __global__ __launch_bounds__(256) void moe_prepare_kernel(const PlanArgs a, const QuantArgs q) {
@@ -926,8 +933,9 @@ __global__ __launch_bounds__(64 * kSumWaves) void moe_down_pairs_kernel(const Pa
 }
 
 struct CombineArgs {
-  const void* slots;  // [tokens * top_k, hidden]: fp32, or fp16 times 2^(e - 127)
-  const uint8_t* slot_e;  // e [tokens * top_k, hidden / 64]
+  const void* slots;      // [positions, hidden]: fp32, or fp16 times 2^(e - 127)
+  const uint8_t* slot_e;  // e [positions, hidden / 64]
+  const int32_t* where;   // the position of each pair of an expert
   const int32_t* ids;
   int64_t id_stride;
   int tokens, top_k, experts, hidden;
@@ -939,10 +947,10 @@ struct CombineArgs {
 constexpr int kCombineAhead = 4;  // slots loaded ahead of their sums
 
 // out[t] (+)= the sum of the token's slots in slot order, in fp32; slots of no
-// expert were never written and are left out (loaded with the others, not used).
+// expert are left out (position 0 is loaded for them, and not used).
 // Bound by the slots' way from HBM.  STREAM: past the caches, where the slots
-// outgrow them: 16384 tokens, 8 slots of 2048 values, 604 MB in 98 us (6.2 TB/s),
-// 116 through the caches.
+// outgrow them: 16384 tokens, 8 slots of 2048 values, 609 MB in 104 us (5.9 TB/s),
+// some 18 more through the caches.
 template <int DT, bool STREAM>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs a) {
   constexpr int kRaw = DT == RIA_DT_F32 ? 2 : 1;  // 16-byte loads of a slot
@@ -956,21 +964,25 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs a) {
   for (int i = 0; i < 8; ++i) s[i] = 0.f;
   for (int j0 = 0; j0 < a.top_k; j0 += kCombineAhead) {
     u32x4 raw[kCombineAhead][kRaw];
-    int id[kCombineAhead];
+    bool on[kCombineAhead];
+    int64_t pos[kCombineAhead];
     uint32_t e[kCombineAhead];
 #pragma unroll
     for (int j = 0; j < kCombineAhead; ++j) {
       const int at = min(j0 + j, a.top_k - 1);
-      const int64_t pair = t * a.top_k + at;
-      id[j] = a.ids[t * a.id_stride + at];
-      if constexpr (DT != RIA_DT_F32) e[j] = a.slot_e[pair * (a.hidden / 64) + c / 64];
-      const u32x4* p = static_cast<const u32x4*>(a.slots) + (pair * a.hidden + c) / 8 * kRaw;
+      const int id = a.ids[t * a.id_stride + at], p = a.where[t * a.top_k + at];
+      on[j] = j0 + j < a.top_k && id >= 0 && id < a.experts;
+      pos[j] = on[j] ? p : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < kCombineAhead; ++j) {
+      if constexpr (DT != RIA_DT_F32) e[j] = a.slot_e[pos[j] * (a.hidden / 64) + c / 64];
+      const u32x4* p = static_cast<const u32x4*>(a.slots) + (pos[j] * a.hidden + c) / 8 * kRaw;
 #pragma unroll
       for (int i = 0; i < kRaw; ++i) raw[j][i] = STREAM ? __builtin_nontemporal_load(p + i) : p[i];
     }
 #pragma unroll
     for (int j = 0; j < kCombineAhead; ++j) {
-      const bool on = j0 + j < a.top_k && id[j] >= 0 && id[j] < a.experts;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float v;
@@ -978,7 +990,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs a) {
           v = __uint_as_float(raw[j][i / 4][i % 4]);
         else
           v = f16_bits_to_f32(static_cast<uint16_t>(raw[j][0][i / 2] >> (16 * (i % 2)))) * x8_scale(e[j]);
-        s[i] = add_rn(s[i], on ? v : 0.f);
+        s[i] = add_rn(s[i], on[j] ? v : 0.f);
       }
     }
   }
@@ -1017,17 +1029,30 @@ static bool moe_by_pairs(int64_t pairs, int experts, int hidden, int inter) {
 // through the caches; 1024 tokens 189, 182 and 204.
 static bool moe_once(int64_t pairs, int experts) { return pairs <= (int64_t)experts * 32; }
 
-// Pairs of one expert that a tile takes.  Same sizes, tiles of 32 / 64: 128
-// tokens 140 / 157 us, 512 tokens 159 / 169, 768 tokens 184 / 182; of 64 / 256:
-// 2048 tokens 243 / 300, 4096 tokens 338 / 357, 8192 tokens 564 / 533.  (fp32 x
-// has no kernel of 256.)
-static int moe_tile(int64_t pairs, int experts, int x_dtype) {
+// Pairs of one expert that a tile takes.  32 or 64 for the weights' way from HBM:
+// (256, 8, 2048, 512) tiles of 32 / 64: 128 tokens 140 / 157 us, 512 tokens 159 /
+// 169, 768 tokens 184 / 182.  64 or 256 by rounds of the gate and up tiles over
+// the card, with the pairs spread evenly and an expert's last tile half full: two
+// tiles of 64 to a CU, one of 256, whose round takes 1.5 times as long.  Measured
+// on both sides, 64 / 256: (256, 8, 2048, 512) 2048 tokens 241 / 285 us, 4096
+// tokens 322 / 340, 6000 tokens 408 / 375, 16384 tokens 963 / 836; (16, 2, 4096,
+// 2048) 512 tokens 134 / 130, 1024 tokens 178 / 150, 3000 tokens 364 / 258; (16,
+// 2, 2048, 1024) 1024 tokens 56 / 68; (60, 4, 1024, 768) 4096 tokens 103 / 122,
+// 6000 tokens 134 / 132; (64, 6, 1024, 512) 1024 tokens 54 / 58, 2048 tokens 74 /
+// 69.  (fp32 x has no kernel of 256.)
+static int moe_tile(int64_t pairs, int experts, int inter, int x_dtype) {
   if (pairs <= (int64_t)experts * 16) return 32;
-  return x_dtype != RIA_DT_F32 && pairs >= (int64_t)experts * 192 ? 256 : 64;
+  if (x_dtype == RIA_DT_F32 || moe_once(pairs, experts)) return 64;
+  const int64_t cus = device_cus(), across = inter / 128;
+  const double each = static_cast<double>(pairs) / experts;
+  const int64_t n64 = static_cast<int64_t>(experts * (each / 64 + 0.5)) * across;
+  const int64_t n256 = static_cast<int64_t>(experts * (each <= 224 ? 1.0 : each / 256 + 0.5)) * across;
+  const int64_t rounds64 = (n64 + 2 * cus - 1) / (2 * cus), rounds256 = (n256 + cus - 1) / cus;
+  return 3 * rounds256 < 2 * rounds64 ? 256 : 64;
 }
 
 struct MoeLayout {
-  int64_t x8, xs, counts, order, tiles, ntiles, act, h8, hs, slots, slot_e, bytes;
+  int64_t x8, xs, counts, order, where, tiles, ntiles, act, h8, hs, slots, slot_e, bytes;
 };
 static MoeLayout moe_layout(int64_t tokens, int top_k, int experts, int hidden, int inter, int x_dtype) {
   MoeLayout l{};
@@ -1045,7 +1070,8 @@ static MoeLayout moe_layout(int64_t tokens, int top_k, int experts, int hidden, 
     l.xs = take(tokens * (hidden / kX8Block) * 4);
     l.counts = take((pairs + kPlanPairs - 1) / kPlanPairs * experts * 4);
     l.order = take(pairs * 4);
-    l.tiles = take(moe_tiles(pairs, experts, moe_tile(pairs, experts, x_dtype)) * static_cast<int64_t>(sizeof(X8Tile)));
+    l.where = take(pairs * 4);
+    l.tiles = take(moe_tiles(pairs, experts, moe_tile(pairs, experts, inter, x_dtype)) * static_cast<int64_t>(sizeof(X8Tile)));
     l.ntiles = take(4);
     l.h8 = take(pairs * inter);
     l.hs = take(pairs * (inter / kX8Block) * 4);
@@ -1224,14 +1250,14 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
     hipLaunchKernelGGL(moe_down_pairs_kernel, dgrid, dim3(64 * kSumWaves), 0, st, p);
     return check_launch(who);
   }
-  const int tile = moe_tile(pairs, d->experts, d->x_dtype);
+  const int tile = moe_tile(pairs, d->experts, d->inter, d->x_dtype);
   const int64_t most = moe_tiles(pairs, d->experts, tile);
   if (most * (std::max(d->hidden, d->inter) / 128) > 0x7ffffff0)
     return set_error(RIA_ERR_INVALID, "%s: too many (token, slot) pairs", who);
   const PlanArgs plan{d->ids, d->ids_row_stride, static_cast<int>(pairs), d->top_k, d->experts,
                       static_cast<int>((pairs + kPlanPairs - 1) / kPlanPairs), tile, static_cast<int32_t*>(at(l.counts)),
-                      static_cast<int32_t*>(at(l.order)), static_cast<X8Tile*>(at(l.tiles)),
-                      static_cast<int32_t*>(at(l.ntiles))};
+                      static_cast<int32_t*>(at(l.order)), static_cast<int32_t*>(at(l.where)),
+                      static_cast<X8Tile*>(at(l.tiles)), static_cast<int32_t*>(at(l.ntiles))};
   const QuantArgs quant{d->tokens * (int64_t)(d->hidden / 8), d->hidden / 8, d->x, d->x_row_stride,
                         static_cast<uint8_t*>(at(l.x8)), static_cast<float*>(at(l.xs))};
   const dim3 pgrid(static_cast<unsigned>(plan.blocks + (quant.units + 255) / 256));
@@ -1243,7 +1269,8 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
     hipLaunchKernelGGL((moe_prepare_kernel<RIA_DT_F32>), pgrid, dim3(256), 0, st, plan, quant);
   if (plan.blocks > 1) hipLaunchKernelGGL(moe_place_kernel, dim3(plan.blocks), dim3(256), 0, st, plan);
   launch_moe_tiles(*d, l, most, tile, st);
-  const CombineArgs c{at(l.slots), static_cast<const uint8_t*>(at(l.slot_e)), d->ids, d->ids_row_stride, d->tokens,
+  const CombineArgs c{at(l.slots), static_cast<const uint8_t*>(at(l.slot_e)),
+                      static_cast<const int32_t*>(at(l.where)), d->ids, d->ids_row_stride, d->tokens,
                       d->top_k, d->experts, d->hidden, d->out, d->out_dtype, d->out_row_stride, d->accumulate != 0,
                       reinterpret_cast<uintptr_t>(d->out) % 16 == 0 && d->out_row_stride % 8 == 0};
   const dim3 grid(static_cast<unsigned>(((int64_t)d->tokens * (d->hidden / 8) + 255) / 256));

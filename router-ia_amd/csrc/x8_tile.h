@@ -172,7 +172,7 @@ __device__ __forceinline__ void quant_unit(const QuantArgs& a, int64_t u) {
 enum X8Mode {
   kX8Dense = 0,  // y [m, n]
   kX8Up = 1,     // an expert's gate and up rows of its tokens, SwiGLU, quantised
-  kX8Down = 2    // an expert's down rows of its pairs, times the router's weight, to the pair's slot
+  kX8Down = 2    // an expert's down rows of its pairs, times the router's weight, to the pairs' positions
 };
 
 struct X8Tile {  // rows of one expert that a workgroup takes: positions first .. first + rows - 1
@@ -198,7 +198,7 @@ struct X8Args {
   int top_k;
   const float* pair_w;
   int64_t pair_w_stride;
-  uint8_t* ye;       // kX8Down with RIA_DT_F16: y holds term / 2^(e - 127), e [pairs, ye_stride] one per 64 features
+  uint8_t* ye;       // kX8Down with RIA_DT_F16: y holds term / 2^(e - 127), e [positions, ye_stride] one per 64 features
   int ye_stride;
   uint8_t* h8;       // kX8Up: [positions, n / 2] e4m3 and its scales [positions, n / 256]
   float* hs;
@@ -569,7 +569,7 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
             scale = x8_inverse(e);
             const int rr = (wt * WT + t) * 32 + l32, g = (n0 + (wf * WF + f0) * 32) / 64;
             if (half == 0 && rr < rows && g < a.ye_stride)
-              a.ye[(int64_t)a.order[first + rr] * a.ye_stride + g] = static_cast<uint8_t>(e);
+              a.ye[(int64_t)(first + rr) * a.ye_stride + g] = static_cast<uint8_t>(e);
           }
         }
 #pragma unroll
@@ -589,8 +589,7 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
           const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
           const int rr = (wt * WT + t) * 32 + r, n = n0 + (wf * WF + f0) * 32 + c;
           if (rr >= rows || n >= a.n) continue;  // n is a multiple of 16: eight features are in or out
-          const int64_t row = MODE == kX8Down ? a.order[first + rr] : first + rr;
-          store_eight<(BM == 256)>(a, row * a.y_stride + n, v);
+          store_eight<(BM == 256)>(a, (int64_t)(first + rr) * a.y_stride + n, v);
         }
       }
     }
