@@ -37,7 +37,8 @@ struct RouteArgs {
   int64_t w_stride;
   int32_t* ids;
   int64_t id_stride;
-  int vec;  // rows and their groups of four logits are aligned for whole loads
+  int vec;   // rows and their groups of four logits are aligned for whole loads
+  int wide;  // scores are compared in 64 bits at once (a wave per token)
 };
 
 // Unsigned integers in the order of floating values: 0 for a taken or absent
@@ -516,9 +517,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_rows_kernel(const 
 }
 
 // One wave per token: scores of few tokens, many experts, groups of no whole
-// lanes.  SCORED as above: 4099 tokens, 256 experts in 8 groups with a bias, 16 us
-// both with the guarded fp32 scores and in 64 bits throughout (some tokens of a
-// batch are chosen again, and 4 us of that show at the end); 16384 tokens 34 and 41.
+// lanes.  SCORED as above, or with a.wide in 64 bits at once.
 template <int XT, int V, bool SCORED>
 __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const RouteArgs a) {
   __shared__ uint64_t group_s[kRouteWaves][64 * V];
@@ -546,17 +545,20 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
   int my_id;
   float my_x;
   if constexpr (SCORED) {
-    float bias[V];
+    bool sure = false;
+    if (!a.wide) {
+      float bias[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) bias[v] = a.bias ? a.bias[min(lane * V + v, e - 1)] : 0.f;
-    uint32_t key[V];
+      for (int v = 0; v < V; ++v) bias[v] = a.bias ? a.bias[min(lane * V + v, e - 1)] : 0.f;
+      uint32_t key[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const uint32_t k = order_key(route_choice(a, x[v], bias[v], top, total));
-      key[v] = lane * V + v < e ? k : 0;
+      for (int v = 0; v < V; ++v) {
+        const uint32_t k = order_key(route_choice(a, x[v], bias[v], top, total));
+        key[v] = lane * V + v < e ? k : 0;
+      }
+      sure = route_select<uint32_t, V, true>(a, lane, key, x, reinterpret_cast<uint32_t*>(group_s[wave]), my_id, my_x);
     }
-    if (!route_select<uint32_t, V, true>(a, lane, key, x, reinterpret_cast<uint32_t*>(group_s[wave]), my_id, my_x))
-      route_select_wide<V>(a, lane, x, top, group_s[wave], my_id, my_x);
+    if (!sure) route_select_wide<V>(a, lane, x, top, group_s[wave], my_id, my_x);
   } else {
     uint32_t key[V];
 #pragma unroll
@@ -593,6 +595,15 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
 // 70; a softmax with a bias 15.2 / 12.5, 22.0 / 21.0, 62 / 78.  (Groups ranked by
 // their largest logit: 4099 tokens 7.3 / 9.3, 65536 tokens 33 / 72.)
 constexpr int kRouteRowsTokens = 12288;
+
+// Where some token is likely to be chosen again (one in fifty is) and the card has
+// room, all of them are chosen in 64 bits at once: the end of a launch is then
+// one choice's chain, not two.  256 experts, 8 groups and a bias, at once / fp32
+// first: 16 tokens 8.5 / 6.6 us or, with one chosen again, 11.6; 256 tokens 9.0 /
+// 11.4, 2048 tokens 10.9 / 12.9, 4099 tokens 17.4 / 15.6, 8192 tokens 24.7 / 21.5;
+// with a bias alone 256 tokens 7.0 / 8.5, 2048 tokens 8.1 / 9.3, 4099 tokens 12.2 /
+// 11.3.
+constexpr int kRouteWideFrom = 32, kRouteWideTo = 3200;
 
 template <int XT, bool SCORED>
 static void launch_route(const RouteArgs& a, hipStream_t st) {
@@ -1182,7 +1193,7 @@ extern "C" int ria_moe_route(int tokens, int experts, int top_k, const void* log
   const bool vec = experts % 4 == 0 && logits_row_stride % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % (4 * size) == 0;
   const RouteArgs a{logits, logits_row_stride, tokens, experts, top_k, bias, scoring == RIA_ROUTE_SIGMOID, num_groups,
                     top_groups, group_score == RIA_ROUTE_GROUP_TOP2, renormalize != 0, s, scale, weights,
-                    weights_row_stride, ids, ids_row_stride, vec};
+                    weights_row_stride, ids, ids_row_stride, vec, tokens >= kRouteWideFrom && tokens < kRouteWideTo};
   // scores need comparing where a bias or a sum of two stands between them and the logits
   const bool scored = bias || (num_groups > 1 && group_score == RIA_ROUTE_GROUP_TOP2);
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -247,13 +247,14 @@ ROUTES = [
 ]
 
 
-MANY = 12288 + 3  # tokens past which a wave takes four of them where scores are compared
+# tokens from which scores are compared in 64 bits at once, in fp32 first again, and by a wave of four tokens
+SOME, MORE, MANY = 32 + 3, 3200 + 3, 12288 + 3
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("case", ROUTES, ids=lambda c: f"t{c['t']}_e{c['e']}_k{c['k']}")
 @pytest.mark.parametrize("masked", [False, True])
-@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("many", [0, SOME, MORE, MANY])
 def test_route_matches_definition(gpu, case, dtype, masked, many):
     c = dict(case)
     t, e, k = c.pop("t"), c.pop("e"), c.pop("k")
@@ -267,7 +268,7 @@ def test_route_matches_definition(gpu, case, dtype, masked, many):
         c["bias"] = torch.randn((e,), generator=gen(3)) * 0.2
     want_w, want_i = route64(x, k, **c)
     if many:  # the same tokens again and again
-        x, want_w, want_i = (v.repeat(MANY // t + 1, 1)[:MANY] for v in (x, want_w, want_i))
+        x, want_w, want_i = (v.repeat(many // t + 1, 1)[:many] for v in (x, want_w, want_i))
     if "bias" in c:
         c["bias"] = c["bias"].to(gpu)
     wide = torch.nn.functional.pad(x, (0, 5)).to(gpu)[:, :cols]
@@ -290,7 +291,7 @@ def test_route_ties_go_to_the_lowest_index(gpu):
     assert i.cpu().tolist() == [[0, 1, 2]]
 
 
-@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("many", [0, SOME, MORE, MANY])
 def test_route_near_ties_follow_64_bits(gpu, many):
     """A bias that brings unlike scores within 1e-9 of each other: fp32 could not order them."""
     announce("moe_route: scores and biases that nearly cancel")
@@ -300,13 +301,13 @@ def test_route_near_ties_follow_64_bits(gpu, many):
     bias = (1.0 - p).float()  # token 0: every choice within fp32 roundings of 1
     want_w, want_i = route64(x, 8, scoring="sigmoid", bias=bias)
     if many:
-        x, want_w, want_i = (v.repeat(MANY // 64 + 1, 1)[:MANY] for v in (x, want_w, want_i))
+        x, want_w, want_i = (v.repeat(many // 64 + 1, 1)[:many] for v in (x, want_w, want_i))
     w, i = K.moe_route(x.to(gpu), 8, scoring="sigmoid", bias=bias.to(gpu))
     assert torch.equal(i.cpu(), want_i)
     torch.testing.assert_close(w.cpu().double(), want_w, rtol=16 * 2.0 ** -24, atol=0)
 
 
-@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("many", [0, SOME, MORE, MANY])
 @pytest.mark.parametrize("groups", [1, 8])
 def test_route_near_ties_in_one_place(gpu, groups, many):
     """The chosen experts and the next one, 1e-9 apart, are neighbours; every other token is far from a tie."""
@@ -318,7 +319,7 @@ def test_route_near_ties_in_one_place(gpu, groups, many):
     c = dict(scoring="sigmoid", num_groups=groups, top_groups=max(groups // 2, 1))
     want_w, want_i = route64(x, 8, bias=bias, **c)
     if many:
-        x, want_w, want_i = (v.repeat(MANY // 37 + 1, 1)[:MANY] for v in (x, want_w, want_i))
+        x, want_w, want_i = (v.repeat(many // 37 + 1, 1)[:many] for v in (x, want_w, want_i))
     w, i = K.moe_route(x.to(gpu), 8, bias=bias.to(gpu), **c)
     assert torch.equal(i.cpu(), want_i)
     torch.testing.assert_close(w.cpu().double(), want_w, rtol=16 * 2.0 ** -24, atol=0)
@@ -347,9 +348,10 @@ def test_route_extreme_logits(gpu):
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups", [1, 2])
-def test_route_extreme_logits_of_many_tokens(gpu, scoring, groups):
+@pytest.mark.parametrize("many", [SOME, MORE, MANY])
+def test_route_extreme_logits_of_many_tokens(gpu, scoring, groups, many):
     """Tokens with infinities and NaN choose the same experts in a large batch as in a small one."""
-    announce(f"moe_route: infinite and NaN logits, {scoring}, {groups} groups, {MANY} tokens")
+    announce(f"moe_route: infinite and NaN logits, {scoring}, {groups} groups, {many} tokens")
     x = torch.randn((7, 64), generator=gen(8))
     x[0, 40], x[0, 9] = math.nan, 5.0
     x[1, 4] = math.inf
@@ -359,10 +361,10 @@ def test_route_extreme_logits_of_many_tokens(gpu, scoring, groups):
     x[5] = -200.0
     c = dict(scoring=scoring, bias=torch.linspace(0, 0.5, 64).to(gpu), num_groups=groups, top_groups=1)
     want_w, want_i = K.moe_route(x.to(gpu), 4, **c)
-    w, i = K.moe_route(x.repeat(MANY // 7 + 1, 1)[:MANY].to(gpu), 4, **c)
-    assert torch.equal(i, want_i.repeat(MANY // 7 + 1, 1)[:MANY])
+    w, i = K.moe_route(x.repeat(many // 7 + 1, 1)[:many].to(gpu), 4, **c)
+    assert torch.equal(i, want_i.repeat(many // 7 + 1, 1)[:many])
     # both sum and divide in fp32, in orders of their own
-    torch.testing.assert_close(w, want_w.repeat(MANY // 7 + 1, 1)[:MANY], rtol=32 * 2.0 ** -24, atol=0, equal_nan=True)
+    torch.testing.assert_close(w, want_w.repeat(many // 7 + 1, 1)[:many], rtol=32 * 2.0 ** -24, atol=0, equal_nan=True)
 
 
 # ----------------------------------------------------------------------------- experts
