@@ -372,6 +372,8 @@ EXPERTS = [  # (tokens, experts, top_k, hidden, inter)
     (1, 8, 2, 256, 128), (1, 16, 8, 2048, 512), (2, 4, 1, 128, 128), (3, 5, 5, 384, 256), (7, 16, 3, 512, 640),
     (17, 3, 2, 256, 128), (40, 33, 4, 256, 384), (130, 6, 2, 640, 256), (200, 2, 2, 256, 128), (300, 40, 6, 512, 128),
     (700, 3, 2, 256, 256), (2100, 5, 2, 256, 128), (400, 20, 1, 384, 256), (900, 24, 2, 640, 128),
+    # tiles of 256 pairs, the last features' half empty; more experts than a planning workgroup has threads
+    (2048, 16, 2, 256, 1024), (1500, 12, 3, 384, 1408), (300, 700, 3, 128, 128), (2000, 1024, 4, 128, 128), (5000, 300, 2, 128, 128),
 ]
 
 
@@ -496,6 +498,23 @@ def test_experts_without_any(gpu, t):
     assert torch.equal(out, keep)
 
 
+@pytest.mark.parametrize("t,e,i", [(4, 5, 128), (60, 16, 128), (300, 8, 128), (2048, 16, 1024)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_experts_overflow_stays_in_its_token(gpu, t, e, i, dtype):
+    """Hidden values that overflow are NaN in e4m3; infinite weights and terms stay infinite or NaN; other tokens keep theirs."""
+    announce(f"moe_experts: overflow in the hidden values and an infinite weight, {t} tokens {dtype}")
+    k, h = 2, 256
+    x, ids, weights, *w = expert_inputs(t, e, k, h, i, dtype, 33 + t)
+    rest = torch.tensor([r for r in range(t) if r not in (1, 2)])
+    want, mag = experts64(x[rest], ids[rest], weights[rest], *w)
+    x[1] *= 1e25
+    weights[2, 0] = math.inf
+    ids[1:3, 0] = 1  # (one expert that is there)
+    out = K.moe_experts(*device((x, ids, weights, *w), gpu)).cpu()
+    assert bool(torch.isnan(out[1]).all()) and not bool(torch.isfinite(out[2]).any())
+    check_experts(out[rest], want, mag, i, dtype)
+
+
 @pytest.mark.parametrize("t", [4, 100])
 def test_experts_nan_and_infinity_stay_in_their_token(gpu, t):
     announce("moe_experts: NaN and infinite activations")
@@ -514,8 +533,8 @@ def test_experts_nan_and_infinity_stay_in_their_token(gpu, t):
 def test_experts_same_inputs_same_bits(gpu):
     """Which place a pair gets in its expert's tiles is left to the order of the counting: the results are not."""
     announce("moe_experts: repeated calls")
-    for t, e, k in ((8, 16, 4), (900, 6, 2), (3000, 6, 2)):
-        a = device(expert_inputs(t, e, k, 256, 256, torch.bfloat16, t), gpu)
+    for t, e, k, i in ((8, 16, 4, 256), (900, 6, 2, 256), (3000, 6, 2, 256), (3000, 12, 2, 1408)):
+        a = device(expert_inputs(t, e, k, 256, i, torch.bfloat16, t), gpu)
         first = K.moe_experts(*a)
         for _ in range(4):
             assert torch.equal(K.moe_experts(*a), first)
