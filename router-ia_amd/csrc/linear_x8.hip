@@ -91,13 +91,16 @@ __global__ __launch_bounds__(64 * NW) void x8_few_kernel(const X8Args a) {
 }
 
 // Some hundred rows: 64 x 64 tiles, the blocks of K dealt to the workgroup's
-// four waves.  Each wave copies its blocks into two halves of LDS of its own
-// and multiplies them with no barrier; the four sums meet in LDS at the end.
-constexpr int kDealWaves = 4;
-template <bool WIDE>
-__global__ __launch_bounds__(64 * kDealWaves) void x8_deal_kernel(const X8Args a) {
+// waves.  Each wave copies a block into LDS of its own and multiplies it with no
+// barrier; the waves' sums meet in LDS at the end.  Bound by the loads' latency
+// and, with two waves a SIMD to cover it, by the CU's 64 bytes a clock into LDS:
+// 333 x 2048 x 4096 to fp32 11.8 us, of it 5 outside the blocks; four waves with
+// two buffers each 14.1.  Operands straight into registers (16 rows x 64 bytes a
+// load, two to four blocks ahead) 25: half lines.
+template <bool WIDE, int NW>
+__global__ __launch_bounds__(64 * NW) void x8_deal_kernel(const X8Args a) {
   constexpr int kStep = 128 * kX8Block;  // 64 rows of w, 64 of x
-  __shared__ __attribute__((aligned(16))) uint8_t lds[kDealWaves * 2 * kStep];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[NW * kStep];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, half = lane >> 5;
@@ -121,17 +124,16 @@ __global__ __launch_bounds__(64 * kDealWaves) void x8_deal_kernel(const X8Args a
   uint32_t xso[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) xso[t] = static_cast<uint32_t>(4 * min(32 * t + l32, rows - 1) * a.xs_stride);
-  uint8_t* own = lds + wave * 2 * kStep;
-  float xs[2][2], sw[2];
-  constexpr int kIssued = 3 + 16;
-  auto issue = [&](int kb, int h) __attribute__((always_inline)) {  // kIssued vector-memory loads
-    xs[h][0] = x8_load_f32(xsr, xso[0], 4 * kb);
-    xs[h][1] = x8_load_f32(xsr, xso[1], 4 * kb);
-    sw[h] = x8_load_f32(wsr, 0, 4 * kb);
+  uint8_t* own = lds + wave * kStep;
+  float xs[2], sw;
+  auto issue = [&](int kb) __attribute__((always_inline)) {
+    xs[0] = x8_load_f32(xsr, xso[0], 4 * kb);
+    xs[1] = x8_load_f32(xsr, xso[1], 4 * kb);
+    sw = x8_load_f32(wsr, 0, 4 * kb);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x8_copy(wr, own + h * kStep + i * 1024, wo[i], kb * kX8Block);
+    for (int i = 0; i < 8; ++i) x8_copy(wr, own + i * 1024, wo[i], kb * kX8Block);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x8_copy(xr, own + h * kStep + (8 + i) * 1024, xo[i], kb * kX8Block);
+    for (int i = 0; i < 8; ++i) x8_copy(xr, own + (8 + i) * 1024, xo[i], kb * kX8Block);
   };
   f32x16 acc[2][2];
 #pragma unroll
@@ -145,8 +147,8 @@ __global__ __launch_bounds__(64 * kDealWaves) void x8_deal_kernel(const X8Args a
     return join_x8(*reinterpret_cast<const u32x4*>(base + r * kX8Block + 16 * (c ^ z)),
                    *reinterpret_cast<const u32x4*>(base + r * kX8Block + 16 * ((c + 1) ^ z)));
   };
-  auto step = [&](int h) __attribute__((always_inline)) {
-    const uint8_t* d = own + h * kStep;
+  auto step = [&]() __attribute__((always_inline)) {
+    const uint8_t* d = own;
     i32x8 b[2][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -162,32 +164,18 @@ __global__ __launch_bounds__(64 * kDealWaves) void x8_deal_kernel(const X8Args a
         for (int i = 0; i < 16; ++i) part[i] = 0.f;
         part = mfma_x8_32<WIDE>(a0, b[t][0], part);
         part = mfma_x8_32<WIDE>(a1, b[t][1], part);
-        const float sc = xs[h][t] * sw[h];
+        const float sc = xs[t] * sw;
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[f][t][i] = fmaf(part[i], sc, acc[f][t][i]);
       }
     }
   };
-  // two blocks a turn, so that the halves are compile-time
-  if (wave < kblocks) {
-    issue(wave, 0);
-    for (int kb = wave; kb < kblocks; kb += 2 * kDealWaves) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (kb + h * kDealWaves >= kblocks) break;
-        const int next = kb + (h + 1) * kDealWaves;
-        if (next < kblocks) {
-          issue(next, h ^ 1);
-          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kIssued) : "memory");  // all but the loads just issued
-        } else {
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
-        step(h);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this half is read before it is copied to again
-      }
-    }
+  for (int kb = wave; kb < kblocks; kb += NW) {
+    issue(kb);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    step();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the block is read before the next is copied over it
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   // sums [wave][row of x][64 features], chunks of four swizzled
   f32x4* sum = reinterpret_cast<f32x4*>(lds);
@@ -202,12 +190,12 @@ __global__ __launch_bounds__(64 * kDealWaves) void x8_deal_kernel(const X8Args a
             f32x4{acc[f][t][4 * q], acc[f][t][4 * q + 1], acc[f][t][4 * q + 2], acc[f][t][4 * q + 3]};
       }
   __syncthreads();
-  for (int u = tid; u < 64 * 16; u += 64 * kDealWaves) {
+  for (int u = tid; u < 64 * 16; u += 64 * NW) {
     const int r = u >> 4, c = u & 15, at_c = c ^ (r & 15);
     if (r >= rows || n0 + 4 * c >= a.n) continue;
     f32x4 s = sum[r * 16 + at_c];
 #pragma unroll
-    for (int j = 1; j < kDealWaves; ++j) s += sum[(j * 64 + r) * 16 + at_c];
+    for (int j = 1; j < NW; ++j) s += sum[(j * 64 + r) * 16 + at_c];
     store_four(a, (int64_t)(m0 + r) * a.y_stride + n0 + 4 * c, s);
   }
 }
@@ -215,12 +203,15 @@ __global__ __launch_bounds__(64 * kDealWaves) void x8_deal_kernel(const X8Args a
 // The kernel of a product.  Up to 32 rows the weights' way from HBM is all there
 // is.  Past that the kernel of the least time by rounds of its tiles over the
 // CUs, in microseconds measured on MI355X (kk = K / 2048): a round of 64 x 64
-// tiles with K dealt to four waves 1.5 + 5 kk; of 128 x 128 tiles 5 + 12 kk with
-// one a CU, 4 + 22.5 kk with two; of 256 x 256 tiles 6 + 32 kk.  Measured on
-// both sides, N = 8192, K = 2048 (64 / 128 / 256 tiles): 256 rows 15.8 / 18.0 /
-// 34.5, 512 rows 28.7 / 19.3 / 35.2, 1024 rows 53 / 29 / 37, 2048 rows 107 / 52 /
-// 42; N = 2048, K = 4096: 512 rows 12.6 / 29.8 / 61, 1536 rows 37 / 31 / 62, 8192
-// rows 193 / 99 / 77.  Wide (fp32 results), 64 / 128: 512 rows 34 / 27, and 15 / 40.
+// tiles with K dealt to the waves 1.6 + 4.6 kk; of 128 x 128 tiles 5 + 12 kk with
+// one a CU, 4 + 22.5 kk with two, between them where some CUs have two; of 256 x
+// 256 tiles 6 + 32 kk.  Measured on both sides, 64 / 128 tiles, N = 8192, K = 2048:
+// 256 rows 14.7 / 18.1, 384 rows 20.9 / 18.9, 2048 rows 107 / 54 (41 with 256);
+// N = 2048, K = 4096: 512 rows 11.1 / 30.0, 1024 rows 22.4 / 30.9, 1536 rows 35.7 /
+// 31.3, 8192 rows 189 / 98 (72 with 256); N = 4096, K = 1024: 512 rows 10.5 / 11.4,
+// 768 rows 15.0 / 11.9.  Wide (fp32 results): N = 8192, K = 2048: 384 rows 23.9 /
+// 26.1, 512 rows 30.0 / 27.6; N = 2048, K = 4096: 512 rows 12.6 / 40.7, 3000 rows
+// 81 / 66.
 enum class X8Plan { kFew, kDeal, kTile128, kTile256 };
 static X8Plan plan_x8(int m, int64_t t256, int64_t t128, int64_t t64, int k, bool wide) {
   if (m <= 32) return X8Plan::kFew;
@@ -229,8 +220,9 @@ static X8Plan plan_x8(int m, int64_t t256, int64_t t128, int64_t t64, int k, boo
   auto rounds = [&](int64_t tiles) { return static_cast<double>((tiles + cus - 1) / cus); };
   const double one = wide ? 7 + 18 * kk : 5 + 12 * kk, two = wide ? 5 + 36 * kk : 4 + 22.5 * kk;
   const int64_t rest = t128 % (2 * cus);
-  const double deal = 2 + rounds(t64) * (wide ? 1.7 + 6.2 * kk : 1.5 + 5 * kk);
-  const double tile128 = 1 + static_cast<double>(t128 / (2 * cus)) * two + (rest == 0 ? 0 : rest <= cus ? one : two);
+  const double last = rest == 0 ? 0 : rest <= cus ? one : two - 0.6 * (two - one) * (2 * cus - rest) / cus;
+  const double deal = 2 + rounds(t64) * (wide ? 1.8 + 5.3 * kk : 1.6 + 4.6 * kk);
+  const double tile128 = 1 + static_cast<double>(t128 / (2 * cus)) * two + last;
   const double tile256 = 2 + rounds(t256) * (6 + 32 * kk);
   if (!wide && tile256 < tile128 && tile256 < deal) return X8Plan::kTile256;
   return tile128 < deal ? X8Plan::kTile128 : X8Plan::kDeal;
@@ -324,10 +316,17 @@ extern "C" int ria_linear_fp8_x8(int m, int n, int k, const void* x, int64_t x_r
     hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, false>), grid(t128), dim3(256), 0, st, a);
   } else if (plan == X8Plan::kTile128) {
     hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, true>), grid(t128), dim3(256), 0, st, a);
-  } else if (!wide) {
-    hipLaunchKernelGGL((x8_deal_kernel<false>), grid(t64), dim3(64 * kDealWaves), 0, st, a);
   } else {
-    hipLaunchKernelGGL((x8_deal_kernel<true>), grid(t64), dim3(64 * kDealWaves), 0, st, a);
+    // a wave for each block of K up to eight: K = 512 with eight waves, half of them idle, takes 0.6 us more
+    const bool deep = k > 4 * kX8Block;
+    if (wide && deep)
+      hipLaunchKernelGGL((x8_deal_kernel<true, 8>), grid(t64), dim3(512), 0, st, a);
+    else if (wide)
+      hipLaunchKernelGGL((x8_deal_kernel<true, 4>), grid(t64), dim3(256), 0, st, a);
+    else if (deep)
+      hipLaunchKernelGGL((x8_deal_kernel<false, 8>), grid(t64), dim3(512), 0, st, a);
+    else
+      hipLaunchKernelGGL((x8_deal_kernel<false, 4>), grid(t64), dim3(256), 0, st, a);
   }
   return check_launch(who);
 }

@@ -216,9 +216,7 @@ __device__ __forceinline__ void x8_copy(__amdgpu_buffer_rsrc_t r, uint8_t* d, ui
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, d, 16, lane_offset, offset, 0, STREAM ? 2 : 0);
 }
 
-// One fp32 through a resource: a vector-memory load for certain (a plain load of
-// an address that is the same in every lane may become a scalar one), where
-// loads in flight are counted.
+// One fp32 through a resource: 32-bit offsets, as the copies beside it have.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t x8_rsrc_f32(const float* p, int64_t count) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, static_cast<int>(static_cast<uint32_t>(4 * count)),
                                            kBufferWord3);
