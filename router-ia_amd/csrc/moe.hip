@@ -39,6 +39,7 @@ struct RouteArgs {
   int64_t id_stride;
   int vec;   // rows and their groups of four logits are aligned for whole loads
   int wide;  // scores are compared in 64 bits at once (a wave per token)
+  int lanes; // lanes of a group, a power of two, where groups are whole lanes (a wave per token), else 0
 };
 
 // Unsigned integers in the order of floating values: 0 for a taken or absent
@@ -200,12 +201,33 @@ __device__ __forceinline__ bool route_select(const RouteArgs& a, int lane, Key (
   const int e = a.experts;
   const Key none = static_cast<Key>(order_key(std::conditional_t<sizeof(Key) == 8, double, float>(-__builtin_inff())));
   bool sure = true;
-  if (a.groups > 1) {
+  // which groups stay open, from each group's rank in lanes step g (and their neighbours, if they hold it too)
+  auto open_groups = [&](Key rank, int g, int step) -> uint64_t {
+    rank = g < a.groups ? rank : 0;
+    int better = 0;  // groups that come before this one
+    for (int j = 0; j < a.groups; ++j) {
+      Key o;
+      if constexpr (sizeof(Key) == 8)
+        o = static_cast<Key>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank >> 32), j * step))) << 32 |
+            static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank), j * step));
+      else
+        o = static_cast<Key>(__builtin_amdgcn_readlane(static_cast<int>(rank), j * step));
+      better += o > rank || (o == rank && j < g);
+    }
+    const bool in = g < a.groups && better < a.top_groups;
+    if constexpr (GUARD) {
+      const Key best_out = uniform(wave_max(in ? Key(0) : rank)), worst_in = uniform(~wave_max(in ? ~rank : Key(0)));
+      if (best_out > none && unsure(worst_in, best_out)) sure = false;
+    }
+    return __ballot(in);
+  };
+  auto rank_of = [&](Key b0, Key b1) { return a.top2 && e > a.groups ? static_cast<Key>(order_key(key_sum(b0, b1))) : b0; };
+  if (a.groups > 1 && !a.lanes) {  // groups of no whole lanes: lane g reads group g's choices
     const int per = e / a.groups;
 #pragma unroll
     for (int v = 0; v < V; ++v) s[lane * V + v] = key[v];
     __builtin_amdgcn_wave_barrier();
-    Key b0 = 0, b1 = 0;  // lane g: group g's best two
+    Key b0 = 0, b1 = 0;  // the group's best two
     const int base = min(lane, a.groups - 1) * per;
     for (int i = 0; i < per; i += 4) {
       Key c[4];
@@ -218,24 +240,7 @@ __device__ __forceinline__ bool route_select(const RouteArgs& a, int lane, Key (
         b0 = max(b0, k);
       }
     }
-    Key rank = a.top2 && per > 1 ? static_cast<Key>(order_key(key_sum(b0, b1))) : b0;
-    rank = lane < a.groups ? rank : 0;
-    int better = 0;  // groups that come before this one
-    for (int j = 0; j < a.groups; ++j) {
-      Key o;
-      if constexpr (sizeof(Key) == 8)
-        o = static_cast<Key>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank >> 32), j))) << 32 |
-            static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(rank), j));
-      else
-        o = static_cast<Key>(__builtin_amdgcn_readlane(static_cast<int>(rank), j));
-      better += o > rank || (o == rank && j < lane);
-    }
-    const bool in = lane < a.groups && better < a.top_groups;
-    const uint64_t open = __ballot(in);
-    if constexpr (GUARD) {
-      const Key best_out = uniform(wave_max(in ? Key(0) : rank)), worst_in = uniform(~wave_max(in ? ~rank : Key(0)));
-      if (best_out > none && unsure(worst_in, best_out)) sure = false;
-    }
+    const uint64_t open = open_groups(rank_of(b0, b1), lane, 1);
     const float inv = 1.f / static_cast<float>(per);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -243,42 +248,71 @@ __device__ __forceinline__ bool route_select(const RouteArgs& a, int lane, Key (
       key[v] = open >> min(g, 63) & 1 ? key[v] : 0;
     }
   }
+  // each lane's experts, the best first (an odd-even merge network; the lower index of equal ones)
+  int at[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) at[v] = v;
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < V; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const int u = i + j, v = i + j + k;
+            const Key ku = key[u], kv = key[v];
+            const int au = at[u], av = at[v];
+            const bool swap = kv > ku || (kv == ku && av < au);
+            key[u] = swap ? kv : ku;
+            key[v] = swap ? ku : kv;
+            at[u] = swap ? av : au;
+            at[v] = swap ? au : av;
+          }
+  if (a.groups > 1 && a.lanes) {  // a group is a.lanes whole lanes: their best two meet by exchanges
+    Key b0 = key[0], b1 = V > 1 ? key[V > 1] : 0;
+    auto meet = [&](Key o0, Key o1) {
+      b1 = max(min(b0, o0), max(b1, o1));
+      b0 = max(b0, o0);
+    };
+    if (a.lanes >= 2) meet(lane_xor<1>(b0), lane_xor<1>(b1));
+    if (a.lanes >= 4) meet(lane_xor<2>(b0), lane_xor<2>(b1));
+    if (a.lanes >= 8) meet(half_mirror(b0), half_mirror(b1));
+    if (a.lanes >= 16) meet(lane_xor<8>(b0), lane_xor<8>(b1));
+    if (a.lanes >= 32) meet(lane_xor<16>(b0), lane_xor<16>(b1));
+    const bool in = open_groups(rank_of(b0, b1), lane / a.lanes, a.lanes) >> lane & 1;
+#pragma unroll
+    for (int v = 0; v < V; ++v) key[v] = in ? key[v] : 0;
+  }
   // top_k times the best that is left; who holds it is scalar work, beside the other waves' vector work
   my_id = -1;
-  my_x = -__builtin_inff();
   Key last = 0;
   for (int j = 0; j < a.top_k + (GUARD ? 1 : 0); ++j) {
-    Key head = key[0];
-#pragma unroll
-    for (int v = 1; v < V; ++v) head = max(head, key[v]);
-    const Key best = uniform(wave_max(head));
+    const Key best = uniform(wave_max(key[0]));
     if (best <= none) break;  // the slots left over keep id -1
     if (GUARD && j > 0 && unsure(last, best)) sure = false;
     if (GUARD && j == a.top_k) break;  // looked at only
     last = best;
-    uint64_t has[V], any = 0;
+    const int from = __builtin_ctzll(__ballot(key[0] == best));  // the lowest lane
+    const int id = from * V + __builtin_amdgcn_readlane(at[0], from);
+    const bool taken = lane == from;
 #pragma unroll
-    for (int v = 0; v < V; ++v) any |= has[v] = __ballot(key[v] == best);
-    const int from = __builtin_ctzll(any);  // the lowest lane, and its first expert of that key
-    int at = V - 1;
-#pragma unroll
-    for (int v = V - 2; v >= 0; --v) at = has[v] >> from & 1 ? v : at;
-    float bx = x[0];
-#pragma unroll
-    for (int v = 1; v < V; ++v) {
-      const float xv = x[v];
-      bx = at == v ? xv : bx;
+    for (int v = 0; v + 1 < V; ++v) {  // (values, not elements, to choose from: no index of the lane's own)
+      const Key here = key[v], next = key[v + 1];
+      const int at_here = at[v], at_next = at[v + 1];
+      key[v] = taken ? next : here;
+      at[v] = taken ? at_next : at_here;
     }
-    bx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(bx), from));
+    key[V - 1] = taken ? 0 : key[V - 1];
+    my_id = lane == j ? id : my_id;
+  }
+  my_x = -__builtin_inff();
+  const int held = max(my_id, 0);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const Key k = key[v];
-      key[v] = lane == from && at == v ? 0 : k;
-    }
-    if (lane == j) {
-      my_id = from * V + at;
-      my_x = bx;
-    }
+  for (int v = 0; v < V; ++v) {
+    const float there = __shfl(x[v], held / V);
+    my_x = my_id >= 0 && held % V == v ? there : my_x;
   }
   return sure;
 }
@@ -316,11 +350,11 @@ __device__ __forceinline__ float route_choice(const RouteArgs& a, float x, float
   return x == -__builtin_inff() ? x : p + bias;
 }
 
-// Whether the token's groups are whole lanes of V experts each, a power of two
-// of them.
-static bool route_groups_fit(const RouteArgs& a, int v) {
+// Lanes of a group, where groups are whole lanes of v experts, a power of two of
+// them; else 0.
+static int route_group_lanes(const RouteArgs& a, int v) {
   const int per = a.experts / a.groups, lanes = per / v;
-  return a.groups == 1 || (per % v == 0 && (lanes & (lanes - 1)) == 0);
+  return per % v == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
 }
 
 // Up to 256 experts and 16 of them chosen: four tokens a wave, 16 lanes each,
@@ -517,7 +551,10 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_rows_kernel(const 
 }
 
 // One wave per token: scores of few tokens, many experts, groups of no whole
-// lanes.  SCORED as above, or with a.wide in 64 bits at once.
+// lanes.  SCORED as above, or with a.wide in 64 bits at once.  Bound by each
+// choice's chain of exchanges: 4099 tokens, 8 of 256 in 4 of 8 groups with a bias
+// and a shared expert, 12.6 us; 16.2 with the choices unsorted in their lanes and
+// the groups' best read back from LDS.
 template <int XT, int V, bool SCORED>
 __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const RouteArgs a) {
   __shared__ uint64_t group_s[kRouteWaves][64 * V];
@@ -589,27 +626,28 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(const Route
 }
 
 // Scores of fewer tokens are chosen by a wave each: its chain of instructions is
-// shorter, and the card is not full.  256 experts, a wave for four tokens / for
-// one: with 8 groups and a bias 4099 tokens 16.7 / 15.9 us, 12000 tokens 23.0 /
-// 27.2, 65536 tokens 60.6 / 102; with a bias alone 13.5 / 11.5, 19.4 / 19.1, 52.4 /
-// 70; a softmax with a bias 15.2 / 12.5, 22.0 / 21.0, 62 / 78.  (Groups ranked by
-// their largest logit: 4099 tokens 7.3 / 9.3, 65536 tokens 33 / 72.)
-constexpr int kRouteRowsTokens = 12288;
+// shorter.  256 experts, a wave for four tokens / for one: with 8 groups and a bias
+// 4099 tokens 15.0 / 12.1 us, 16384 tokens 24.4 / 23.8, 65536 tokens 61 / 74; with
+// a bias alone 15.7 / 9.9, 21.6 / 19.5, 55 / 59; a softmax with a bias 15.0 / 11.6,
+// 27.2 / 24.4, 65 / 75.
+constexpr int kRouteRowsTokens = 32768;
 
 // Where some token is likely to be chosen again (one in fifty is) and the card has
 // room, all of them are chosen in 64 bits at once: the end of a launch is then
-// one choice's chain, not two.  256 experts, 8 groups and a bias, at once / fp32
-// first: 16 tokens 8.5 / 6.6 us or, with one chosen again, 11.6; 256 tokens 9.0 /
-// 11.4, 2048 tokens 10.9 / 12.9, 4099 tokens 17.4 / 15.6, 8192 tokens 24.7 / 21.5;
-// with a bias alone 256 tokens 7.0 / 8.5, 2048 tokens 8.1 / 9.3, 4099 tokens 12.2 /
-// 11.3.
+// one choice's chain, not two.  256 experts, at once / fp32 first, with 8 groups
+// and a bias: 16 tokens 7.0 / 6.6 us or, with one chosen again, 8.4; 512 tokens
+// 7.1 / 9.2, 2048 tokens 8.2 / 10.1, 4099 tokens 11.9 / 12.0, 8192 tokens 17.0 /
+// 15.9; with a bias alone 512 tokens 7.0 / 7.6, 2048 tokens 7.2 / 8.7, 4099 tokens
+// 10.1 / 9.9, 8192 tokens 14.5 / 12.8.
 constexpr int kRouteWideFrom = 32, kRouteWideTo = 3200;
 
 template <int XT, bool SCORED>
-static void launch_route(const RouteArgs& a, hipStream_t st) {
+static void launch_route(RouteArgs a, hipStream_t st) {
   const bool few = a.top_k <= 8;
   const int per_lane = a.experts <= 64 ? 4 : a.experts <= 128 && few ? 8 : 16;
-  if (a.experts <= 256 && a.top_k <= 16 && route_groups_fit(a, per_lane) && (!SCORED || a.tokens >= kRouteRowsTokens)) {
+  if (a.experts <= 256 && a.top_k <= 16 && (a.groups == 1 || route_group_lanes(a, per_lane)) &&
+      (!SCORED || a.tokens >= kRouteRowsTokens)) {
+    a.lanes = route_group_lanes(a, per_lane / 4);  // of a token that the whole wave chooses again
     const dim3 grid((a.tokens + 4 * kRouteWaves - 1) / (4 * kRouteWaves)), block(64 * kRouteWaves);
     if (per_lane == 4)
       hipLaunchKernelGGL((moe_route_rows_kernel<XT, 4, 16, SCORED>), grid, block, 0, st, a);
@@ -622,12 +660,13 @@ static void launch_route(const RouteArgs& a, hipStream_t st) {
     return;
   }
   const dim3 grid((a.tokens + kRouteWaves - 1) / kRouteWaves), block(64 * kRouteWaves);
-  const int v = (a.experts + 63) / 64;
-  if (v <= 1)
+  const int v = a.experts <= 64 ? 1 : a.experts <= 256 ? 4 : a.experts <= 512 ? 8 : 16;
+  a.lanes = route_group_lanes(a, v);
+  if (v == 1)
     hipLaunchKernelGGL((moe_route_kernel<XT, 1, SCORED>), grid, block, 0, st, a);
-  else if (v <= 4)
+  else if (v == 4)
     hipLaunchKernelGGL((moe_route_kernel<XT, 4, SCORED>), grid, block, 0, st, a);
-  else if (v <= 8)
+  else if (v == 8)
     hipLaunchKernelGGL((moe_route_kernel<XT, 8, SCORED>), grid, block, 0, st, a);
   else
     hipLaunchKernelGGL((moe_route_kernel<XT, 16, SCORED>), grid, block, 0, st, a);
@@ -1193,7 +1232,7 @@ extern "C" int ria_moe_route(int tokens, int experts, int top_k, const void* log
   const bool vec = experts % 4 == 0 && logits_row_stride % 4 == 0 && reinterpret_cast<uintptr_t>(logits) % (4 * size) == 0;
   const RouteArgs a{logits, logits_row_stride, tokens, experts, top_k, bias, scoring == RIA_ROUTE_SIGMOID, num_groups,
                     top_groups, group_score == RIA_ROUTE_GROUP_TOP2, renormalize != 0, s, scale, weights,
-                    weights_row_stride, ids, ids_row_stride, vec, tokens >= kRouteWideFrom && tokens < kRouteWideTo};
+                    weights_row_stride, ids, ids_row_stride, vec, tokens >= kRouteWideFrom && tokens < kRouteWideTo, 0};
   // scores need comparing where a bias or a sum of two stands between them and the logits
   const bool scored = bias || (num_groups > 1 && group_score == RIA_ROUTE_GROUP_TOP2);
   hipStream_t st = static_cast<hipStream_t>(stream);

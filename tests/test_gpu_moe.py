@@ -244,11 +244,17 @@ ROUTES = [
     dict(t=50, e=256, k=8, bias=True, num_groups=64, top_groups=9),
     dict(t=50, e=96, k=3, bias=True, num_groups=2, top_groups=1),
     dict(t=50, e=256, k=8, scoring="softmax", num_groups=2, top_groups=1, group_score="max", renormalize=False),
+    # groups of 1, 4, 8, 16 and 32 lanes of a wave that takes one token
+    dict(t=20, e=60, k=7, scoring="sigmoid", bias=True, num_groups=60, top_groups=20),
+    dict(t=20, e=256, k=20, bias=True, num_groups=16, top_groups=5),
+    dict(t=20, e=512, k=9, bias=True, num_groups=8, top_groups=3),
+    dict(t=20, e=1024, k=11, scoring="sigmoid", bias=True, num_groups=4, top_groups=2),
+    dict(t=20, e=1024, k=32, num_groups=2, top_groups=1, group_score="max"),
 ]
 
 
 # tokens from which scores are compared in 64 bits at once, in fp32 first again, and by a wave of four tokens
-SOME, MORE, MANY = 32 + 3, 3200 + 3, 12288 + 3
+SOME, MORE, MANY = 32 + 3, 3200 + 3, 32768 + 3
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
