@@ -9,6 +9,8 @@
 // 128 values of a row, found as they come.  The reference multiplies in fp16
 // (qwen36_attention_cache.py:232-247), which linear_fp8.hip reproduces; here
 // both operands stay in 8 bits and the matrix cores run at twice the rate.
+#include <algorithm>
+
 #include "x8_tile.h"
 
 namespace ria {
@@ -204,28 +206,39 @@ __global__ __launch_bounds__(64 * NW) void x8_deal_kernel(const X8Args a) {
 // is.  Past that the kernel of the least time by rounds of its tiles over the
 // CUs, in microseconds measured on MI355X (kk = K / 2048): a round of 64 x 64
 // tiles with K dealt to the waves 1.6 + 4.6 kk; of 128 x 128 tiles 5 + 12 kk with
-// one a CU, 4 + 22.5 kk with two, between them where some CUs have two; of 256 x
-// 256 tiles 6 + 32 kk.  Measured on both sides, 64 / 128 tiles, N = 8192, K = 2048:
+// one a CU, 4 + 22.5 kk with two, between them where some CUs have two, 3 + 28 kk
+// with three of one LDS buffer (no rounds: they start one by one); of 256 x 256
+// tiles 6 + 32 kk.  Measured on both sides, 64 / 128 tiles, N = 8192, K = 2048:
 // 256 rows 14.7 / 18.1, 384 rows 20.9 / 18.9, 2048 rows 107 / 54 (41 with 256);
 // N = 2048, K = 4096: 512 rows 11.1 / 30.0, 1024 rows 22.4 / 30.9, 1536 rows 35.7 /
 // 31.3, 8192 rows 189 / 98 (72 with 256); N = 4096, K = 1024: 512 rows 10.5 / 11.4,
 // 768 rows 15.0 / 11.9.  Wide (fp32 results): N = 8192, K = 2048: 384 rows 23.9 /
 // 26.1, 512 rows 30.0 / 27.6; N = 2048, K = 4096: 512 rows 12.6 / 40.7, 3000 rows
-// 81 / 66.
-enum class X8Plan { kFew, kDeal, kTile128, kTile256 };
+// 81 / 66.  Tiles of 128 with one buffer / two: N = 8192, K = 2048: 512 rows 23.5 /
+// 19.7, 1024 rows 26.5 / 27.2, 3000 rows 76 / 78; N = 2048, K = 4096: 2048 rows 41 /
+// 32, 3000 rows 43.5 / 47, 4096 rows 46 / 51; N = 4096, K = 1024: 2048 rows 17.2 /
+// 16.9, 3000 rows 22.5 / 22.5.
+enum class X8Plan { kFew, kDeal, kTile128, kTile128Many, kTile256 };
 static X8Plan plan_x8(int m, int64_t t256, int64_t t128, int64_t t64, int k, bool wide) {
   if (m <= 32) return X8Plan::kFew;
   const int64_t cus = device_cus();
   const double kk = k / 2048.0;
   auto rounds = [&](int64_t tiles) { return static_cast<double>((tiles + cus - 1) / cus); };
   const double one = wide ? 7 + 18 * kk : 5 + 12 * kk, two = wide ? 5 + 36 * kk : 4 + 22.5 * kk;
-  const int64_t rest = t128 % (2 * cus);
-  const double last = rest == 0 ? 0 : rest <= cus ? one : two - 0.6 * (two - one) * (2 * cus - rest) / cus;
   const double deal = 2 + rounds(t64) * (wide ? 1.8 + 5.3 * kk : 1.6 + 4.6 * kk);
-  const double tile128 = 1 + static_cast<double>(t128 / (2 * cus)) * two + last;
   const double tile256 = 2 + rounds(t256) * (6 + 32 * kk);
+  const bool many = !wide && t128 > cus;
+  double tile128;
+  if (many) {
+    tile128 = std::max(0.9 * two, 4 + (3 + 28 * kk) * static_cast<double>(t128) / static_cast<double>(3 * cus));
+  } else {
+    const int64_t rest = t128 % (2 * cus);
+    const double last = rest == 0 ? 0 : rest <= cus ? one : two - 0.6 * (two - one) * (2 * cus - rest) / cus;
+    tile128 = 1 + static_cast<double>(t128 / (2 * cus)) * two + last;
+  }
   if (!wide && tile256 < tile128 && tile256 < deal) return X8Plan::kTile256;
-  return tile128 < deal ? X8Plan::kTile128 : X8Plan::kDeal;
+  if (deal <= tile128) return X8Plan::kDeal;
+  return many ? X8Plan::kTile128Many : X8Plan::kTile128;
 }
 
 bool x8_dtype_ok(int dt) { return dt == RIA_DT_BF16 || dt == RIA_DT_F16 || dt == RIA_DT_F32; }
@@ -312,6 +325,8 @@ extern "C" int ria_linear_fp8_x8(int m, int n, int k, const void* x, int64_t x_r
       hipLaunchKernelGGL((x8_few_kernel<2, 4>), few, dim3(256), 0, st, a);
   } else if (plan == X8Plan::kTile256) {
     hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 4, 2, 2, 4, false>), grid(t256), dim3(512), 0, st, a);
+  } else if (plan == X8Plan::kTile128Many) {
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, false, false, 3>), grid(t128), dim3(256), 0, st, a);
   } else if (plan == X8Plan::kTile128 && !wide) {
     hipLaunchKernelGGL((x8_tile_kernel<kX8Dense, 2, 2, 2, 2, false>), grid(t128), dim3(256), 0, st, a);
   } else if (plan == X8Plan::kTile128) {

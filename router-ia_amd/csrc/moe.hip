@@ -1079,6 +1079,11 @@ static bool moe_by_pairs(int64_t pairs, int experts, int hidden, int inter) {
 // through the caches; 1024 tokens 189, 182 and 204.
 static bool moe_once(int64_t pairs, int experts) { return pairs <= (int64_t)experts * 32; }
 
+// Gate and up tiles of 64 pairs, with an expert's last one half full.
+static int64_t moe_tiles64(int64_t pairs, int experts, int inter) {
+  return static_cast<int64_t>(static_cast<double>(pairs) / 64 + 0.5 * experts) * (inter / 128);
+}
+
 // Pairs of one expert that a tile takes.  32 or 64 for the weights' way from HBM:
 // (256, 8, 2048, 512) tiles of 32 / 64: 128 tokens 140 / 157 us, 512 tokens 159 /
 // 169, 768 tokens 184 / 182.  64 or 256 by rounds of the gate and up tiles over
@@ -1095,7 +1100,7 @@ static int moe_tile(int64_t pairs, int experts, int inter, int x_dtype) {
   if (x_dtype == RIA_DT_F32 || moe_once(pairs, experts)) return 64;
   const int64_t cus = device_cus(), across = inter / 128;
   const double each = static_cast<double>(pairs) / experts;
-  const int64_t n64 = static_cast<int64_t>(experts * (each / 64 + 0.5)) * across;
+  const int64_t n64 = moe_tiles64(pairs, experts, inter);
   const int64_t n256 = static_cast<int64_t>(experts * (each <= 224 ? 1.0 : each / 256 + 0.5)) * across;
   const int64_t rounds64 = (n64 + 2 * cus - 1) / (2 * cus), rounds256 = (n256 + cus - 1) / cus;
   return 3 * rounds256 < 2 * rounds64 ? 256 : 64;
@@ -1152,7 +1157,11 @@ static void launch_moe_tiles(const ria_moe_experts_desc& d, const MoeLayout& l, 
   up.h8 = static_cast<uint8_t*>(at(l.h8));
   up.hs = static_cast<float*>(at(l.hs));
   up.m = d.tokens;
-  const bool wide = d.x_dtype == RIA_DT_F32, once = moe_once((int64_t)d.tokens * d.top_k, d.experts);
+  const int64_t pairs = (int64_t)d.tokens * d.top_k;
+  const bool wide = d.x_dtype == RIA_DT_F32, once = moe_once(pairs, d.experts);
+  // tiles of 64 in 16-bit x: one LDS buffer where there are more than two for a CU.  (256, 8, 2048, 512) 4096 tokens
+  // 311 us, 322 with two buffers, (60, 4, 1024, 768) 4096 tokens 100 and 104; (8, 2, 4096, 1024) 512 tokens 72 and 60
+  const bool many = moe_tiles64(pairs, d.experts, d.inter) > 2 * (int64_t)device_cus();
   auto grid_of = [&](int feature_tiles) { return dim3(static_cast<unsigned>((most * feature_tiles + 7) / 8 * 8)); };
   if (tile == 32)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 1, 4, 1, true, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
@@ -1162,6 +1171,8 @@ static void launch_moe_tiles(const ria_moe_experts_desc& d, const MoeLayout& l, 
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   else if (tile == 256)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 4, 2, 2, 4, false>), grid_of(d.inter / 128), dim3(512), 0, st, up);
+  else if (many)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false, false, 3>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   else
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   X8Args dn = up;
@@ -1189,6 +1200,8 @@ static void launch_moe_tiles(const ria_moe_experts_desc& d, const MoeLayout& l, 
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, true>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
   else if (tile == 256)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 4, 2, 2, 4, false>), grid_of((d.hidden + 255) / 256), dim3(512), 0, st, dn);
+  else if (many)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, false, false, 4>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
   else
     hipLaunchKernelGGL((x8_tile_kernel<kX8Down, 2, 1, 2, 2, false>), grid_of(d.hidden / 128), dim3(256), 0, st, dn);
 }

@@ -300,11 +300,16 @@ __device__ __forceinline__ int x8_order(int b, int total) {
 // Large tiles (4, 2, 2, 4: 256 x 256, one workgroup a CU) are bound by the matrix
 // cores at the clock they allow, beside 64 KB of LDS copies, 128 KB of LDS reads
 // and the scaling's FMAs a step: some 2 us a step, 6 outside the steps.  16384 x
-// 8192 x 2048 to fp16 in 300 us, 1.83 PFLOP/s; 128 x 256 tiles with one LDS
+// 8192 x 2048 to fp16 in 295 us, 1.86 PFLOP/s; 128 x 256 tiles with one LDS
 // buffer, two workgroups a CU: 330 (and the experts' products the same as now).
 // Small tiles (32 or 64 rows) are bound by the weights' way from HBM.
-template <int MODE, int WF, int WT, int NF, int NT, bool WIDE, bool STREAM = false>
-__global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
+//
+// ONE: one LDS buffer, and registers for ONE waves a SIMD: a step's copies are
+// covered by the CU's other workgroups, where there are more than two for it.
+// 4096 x 2048 x 4096 in tiles of 128 x 128: 46 us, 51 with two buffers; but with
+// one tile a CU (2048 x 2048 x 4096) 41 and 32.
+template <int MODE, int WF, int WT, int NF, int NT, bool WIDE, bool STREAM = false, int ONE = 0>
+__global__ __launch_bounds__(64 * NF * NT, ONE ? ONE : 1) void x8_tile_kernel(const X8Args a) {
   constexpr int NW = NF * NT;
   constexpr int BN = 32 * WF * NF, BM = 32 * WT * NT;
   constexpr int WL = BN / 8 / NW, XL = BM / 8 / NW;  // 1 KiB copies of a wave per step
@@ -313,7 +318,7 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
   constexpr int kStep = (BN + BM) * kX8Block;  // bytes of a step
   constexpr int kPitch = 64 + 4;               // fp32 values of a row that a wave stages for its stores
   constexpr int kStage = 32 * kPitch * 4;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kStep > NW * kStage ? 2 * kStep : NW * kStage];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[(ONE ? 1 : 2) * kStep > NW * kStage ? (ONE ? 1 : 2) * kStep : NW * kStage];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wf = wave % NF, wt = wave / NF;
@@ -382,7 +387,7 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
     xo[i] = static_cast<uint32_t>((x_row(r) - x0) * a.x_stride) + 16 * ((lane & 7) ^ ((r >> 1) & 7));
   }
   auto issue = [&](int kb) __attribute__((always_inline)) {
-    uint8_t* d = lds + (kb & 1) * kStep;
+    uint8_t* d = lds + (ONE ? 0 : (kb & 1) * kStep);
 #pragma unroll
     for (int i = 0; i < WL; ++i) x8_copy<STREAM>(wr, d + (wave * WL + i) * 1024, wo[i], kb * kX8Block);
 #pragma unroll
@@ -440,29 +445,37 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
     }
     if (kb + 1 < kblocks) {
       load_scales(kb + 1);
-      issue(kb + 1);
+      if (!ONE) issue(kb + 1);
     }
-    if (!live) continue;
-    const uint8_t* d = lds + (kb & 1) * kStep;
-    i32x8 b[WT][2];
+    if constexpr (!ONE) {
+      if (!live) continue;
+    }
+    if (!ONE || live) {
+      const uint8_t* d = lds + (ONE ? 0 : (kb & 1) * kStep);
+      i32x8 b[WT][2];
 #pragma unroll
-    for (int t = 0; t < WT; ++t)
+      for (int t = 0; t < WT; ++t)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) b[t][s] = operand(d + BN * kX8Block, (wt * WT + t) * 32 + l32, s);
+        for (int s = 0; s < 2; ++s) b[t][s] = operand(d + BN * kX8Block, (wt * WT + t) * 32 + l32, s);
 #pragma unroll
-    for (int f = 0; f < WF; ++f) {
-      const i32x8 a0 = operand(d, (wf * WF + f) * 32 + l32, 0), a1 = operand(d, (wf * WF + f) * 32 + l32, 1);
+      for (int f = 0; f < WF; ++f) {
+        const i32x8 a0 = operand(d, (wf * WF + f) * 32 + l32, 0), a1 = operand(d, (wf * WF + f) * 32 + l32, 1);
 #pragma unroll
-      for (int t = 0; t < WT; ++t) {
-        f32x16 part;
+        for (int t = 0; t < WT; ++t) {
+          f32x16 part;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) part[i] = 0.f;
-        part = mfma_x8_32<WIDE>(a0, b[t][0], part);
-        part = mfma_x8_32<WIDE>(a1, b[t][1], part);
-        const float sc = f < WF / 2 ? s0[t] : s1[t];
+          for (int i = 0; i < 16; ++i) part[i] = 0.f;
+          part = mfma_x8_32<WIDE>(a0, b[t][0], part);
+          part = mfma_x8_32<WIDE>(a1, b[t][1], part);
+          const float sc = f < WF / 2 ? s0[t] : s1[t];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[f][t][i] = fmaf(part[i], sc, acc[f][t][i]);
+          for (int i = 0; i < 16; ++i) acc[f][t][i] = fmaf(part[i], sc, acc[f][t][i]);
+        }
       }
+    }
+    if (ONE && kb + 1 < kblocks) {
+      __syncthreads();  // the step is read before the next is copied over it
+      issue(kb + 1);
     }
   }
   __syncthreads();
@@ -472,7 +485,7 @@ __global__ __launch_bounds__(64 * NF * NT) void x8_tile_kernel(const X8Args a) {
     // waves' parts of its largest value meet in LDS
     float* top = reinterpret_cast<float*>(lds);               // [NF][BM]
     uint8_t* stage = lds + NF * BM * 4;                       // [BM][128] quantised, chunks swizzled
-    static_assert(NF * BM * 4 + BM * 128 <= 2 * kStep, "both fit");
+    static_assert(NF * BM * 4 + BM * 128 <= (ONE ? 1 : 2) * kStep, "both fit");
     constexpr int HF = WF / 2;
 #pragma unroll
     for (int t = 0; t < WT; ++t) {

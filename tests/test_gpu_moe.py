@@ -161,6 +161,7 @@ LINEAR = [  # (m, n, k)
     (1, 16, 128), (1, 8192, 2048), (2, 48, 256), (5, 400, 1152), (16, 512, 2048), (17, 2048, 4096), (33, 144, 128),
     (64, 1040, 640), (100, 2048, 512), (129, 272, 2048), (200, 1536, 384), (300, 2048, 4096), (513, 784, 896),
     (1025, 4112, 256), (40, 96, 128), (70, 80, 384), (4001, 4080, 384),
+    (1500, 3088, 512), (2001, 8176, 1152),
 ]
 
 
@@ -380,6 +381,7 @@ EXPERTS = [  # (tokens, experts, top_k, hidden, inter)
     (700, 3, 2, 256, 256), (2100, 5, 2, 256, 128), (400, 20, 1, 384, 256), (900, 24, 2, 640, 128),
     # tiles of 256 pairs, the last features' half empty; more experts than a planning workgroup has threads
     (2048, 16, 2, 256, 1024), (1500, 12, 3, 384, 1408), (300, 700, 3, 128, 128), (2000, 1024, 4, 128, 128), (5000, 300, 2, 128, 128),
+    (1700, 40, 3, 256, 1024),  # tiles of 64 pairs, more than two a CU
 ]
 
 
