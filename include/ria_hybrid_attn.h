@@ -767,7 +767,7 @@ int ria_moe_route(int tokens, int experts, int top_k, const void* logits, int lo
  * with a scale per 64, so x_dtype's range is theirs); their sum is fp32, rounded
  * once to out_dtype, or with accumulate added to out (fp32).  With an fp32 x
  * both products are summed in fp32 from widened operands, as fp32 results of
- * ria_linear_fp8_x8 are.  Slots whose id is outside [0, experts) add
+ * ria_linear_fp8_x8 are, with an fp16 x the first.  Slots whose id is outside [0, experts) add
  * nothing (a token without any gets 0); an expert may come twice in a row.
  *   x     [tokens, hidden] of x_dtype, 16-byte aligned, row stride a multiple of 8
  *   w13   [experts, 2 inter, hidden] e4m3, gate rows first; w13_scale_inv f32

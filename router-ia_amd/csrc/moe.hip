@@ -1000,7 +1000,7 @@ constexpr int kCombineAhead = 4;  // slots loaded ahead of their sums
 // expert are left out (position 0 is loaded for them, and not used).
 // Bound by the slots' way from HBM.  STREAM: past the caches, where the slots
 // outgrow them: 16384 tokens, 8 slots of 2048 values, 609 MB in 104 us (5.9 TB/s),
-// some 18 more through the caches.
+// some 18 more through the caches; 33 MB of slots take the same either way.
 template <int DT, bool STREAM>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs a) {
   constexpr int kRaw = DT == RIA_DT_F32 ? 2 : 1;  // 16-byte loads of a slot
@@ -1094,10 +1094,10 @@ static int64_t moe_tiles64(int64_t pairs, int experts, int inter) {
 // 2048) 512 tokens 134 / 130, 1024 tokens 178 / 150, 3000 tokens 364 / 258; (16,
 // 2, 2048, 1024) 1024 tokens 56 / 68; (60, 4, 1024, 768) 4096 tokens 103 / 122,
 // 6000 tokens 134 / 132; (64, 6, 1024, 512) 1024 tokens 54 / 58, 2048 tokens 74 /
-// 69.  (fp32 x has no kernel of 256.)
+// 69.  (Only a bf16 x has kernels of 256: widened operands' registers do not fit.)
 static int moe_tile(int64_t pairs, int experts, int inter, int x_dtype) {
   if (pairs <= (int64_t)experts * 16) return 32;
-  if (x_dtype == RIA_DT_F32 || moe_once(pairs, experts)) return 64;
+  if (x_dtype != RIA_DT_BF16 || moe_once(pairs, experts)) return 64;
   const int64_t cus = device_cus(), across = inter / 128;
   const double each = static_cast<double>(pairs) / experts;
   const int64_t n64 = moe_tiles64(pairs, experts, inter);
@@ -1159,18 +1159,23 @@ static void launch_moe_tiles(const ria_moe_experts_desc& d, const MoeLayout& l, 
   up.m = d.tokens;
   const int64_t pairs = (int64_t)d.tokens * d.top_k;
   const bool wide = d.x_dtype == RIA_DT_F32, once = moe_once(pairs, d.experts);
-  // tiles of 64 in 16-bit x: one LDS buffer where there are more than two for a CU.  (256, 8, 2048, 512) 4096 tokens
+  // tiles of 64 in e4m3 products: one LDS buffer where there are more than two for a CU.  (256, 8, 2048, 512) 4096 tokens
   // 311 us, 322 with two buffers, (60, 4, 1024, 768) 4096 tokens 100 and 104; (8, 2, 4096, 1024) 512 tokens 72 and 60
   const bool many = moe_tiles64(pairs, d.experts, d.inter) > 2 * (int64_t)device_cus();
   auto grid_of = [&](int feature_tiles) { return dim3(static_cast<unsigned>((most * feature_tiles + 7) / 8 * 8)); };
+  // Where the e4m3 products' 3e-5 carry a hidden value over a rounding border of e4m3, it moves by up to 2^-3: results
+  // are 1e-3 off (2-norm) by that, four times an fp16 rounding, half a bf16 one.  So only a bf16 x takes them here; an
+  // fp16 one's gate and up rows are summed from widened operands, as an fp32 one's are (16384 tokens, 8 of 256 experts
+  // of 2048 x 512: 1121 us, 840 without; 2048 tokens 249 and 240).
+  const bool wide_up = d.x_dtype != RIA_DT_BF16;
   if (tile == 32)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 1, 4, 1, true, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   else if (once)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
-  else if (wide)
-    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   else if (tile == 256)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 4, 2, 2, 4, false>), grid_of(d.inter / 128), dim3(512), 0, st, up);
+  else if (wide_up)
+    hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, true>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   else if (many)
     hipLaunchKernelGGL((x8_tile_kernel<kX8Up, 2, 2, 4, 1, false, false, 3>), grid_of(d.inter / 128), dim3(256), 0, st, up);
   else
@@ -1339,7 +1344,7 @@ extern "C" int ria_moe_experts(const ria_moe_experts_desc* d, void* stream) {
   const dim3 grid(static_cast<unsigned>(((int64_t)d->tokens * (d->hidden / 8) + 255) / 256));
   if (d->x_dtype == RIA_DT_F32)
     hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F32, false>), grid, dim3(256), 0, st, c);
-  else if (tile == 256)
+  else if (pairs * d->hidden * 2 >= int64_t(32) << 20)
     hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F16, true>), grid, dim3(256), 0, st, c);
   else
     hipLaunchKernelGGL((moe_combine_kernel<RIA_DT_F16, false>), grid, dim3(256), 0, st, c);

@@ -1328,7 +1328,8 @@ def moe_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, w13: 
     int32 and weights fp32 [T, k] as moe_route gives them (ids outside the
     experts add nothing); w13 [E, 2 I, H] (gate rows first) and w2 [E, H, I]
     float8_e4m3fn with fp32 scales per 128x128 block, H and I multiples of
-    128.  A slot's terms are kept to 11 bits or more (in fp32 with an fp32 x),
+    128.  A bf16 x takes the e4m3 matrix products, 3e-5 off, throughout large
+    batches.  A slot's terms are kept to 11 bits or more (in fp32 with an fp32 x),
     their fp32 sum is rounded once to out's dtype.  Returns / fills out [T, H]
     (x's dtype unless out_dtype or out says otherwise); with ``accumulate`` the
     fp32 ``out`` receives out + the sum.

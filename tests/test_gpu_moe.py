@@ -541,7 +541,7 @@ def test_experts_nan_and_infinity_stay_in_their_token(gpu, t):
 def test_experts_same_inputs_same_bits(gpu):
     """Which place a pair gets in its expert's tiles is left to the order of the counting: the results are not."""
     announce("moe_experts: repeated calls")
-    for t, e, k, i in ((8, 16, 4, 256), (900, 6, 2, 256), (3000, 6, 2, 256), (3000, 12, 2, 1408)):
+    for t, e, k, i in ((8, 16, 4, 256), (900, 6, 2, 256), (3000, 6, 2, 256), (3000, 12, 2, 1408), (9000, 6, 4, 256)):
         a = device(expert_inputs(t, e, k, 256, i, torch.bfloat16, t), gpu)
         first = K.moe_experts(*a)
         for _ in range(4):
